@@ -360,6 +360,112 @@ nq_status_t nq_mixed_precision_matmul(const float* a, const int8_t* b, const flo
    kernels here need no workspace). */
 size_t nq_fp8_gemm_workspace_size(int m, int k, int n);
 
+/* ---- microscaled 4-bit formats ------------------------------------------------
+ * No reference counterpart (its lowest precision is 8 bits).  A rows x cols
+ * matrix in 4 bits: E2M1 elements (0, .5, 1, 1.5, 2, 3, 4, 6 and negatives),
+ * scaled in blocks along a row:
+ *   NQ_MXFP4  blocks of 32, scale 2^(floor(log2 amax_block) - 2) (E8M0 byte,
+ *             at least 2^-127), code = E2M1(x / scale);
+ *   NQ_NVFP4  blocks of 16 and one fp32 scale a row.  A = max(amax_row,
+ *             2688 * 2^-110); row scale A / 2688 (1.0 for an all-zero row);
+ *             block scale s = E4M3(448 amax_block / A); code =
+ *             E2M1(2688 x / (s A)), 0 where s is 0.
+ * Roundings are to nearest even, saturating.  The sign of a code that is zero
+ * is not specified.  An infinity or NaN gives MXFP4 a block scale NaN (0xFF)
+ * and NVFP4 a row scale NaN; the codes under it are zero.
+ * Value of an element: code * block scale [* row scale].
+ *
+ * Storage:
+ *   codes         rows of nq_mx4_row_bytes(cols) = 16 * ceil(cols / 32) bytes,
+ *                 two codes a byte (even column in the low nibble), zero behind
+ *                 the last column; 16-byte aligned;
+ *   block scales  nq_mx4_scale_bytes(rows, cols, fmt) bytes in 512-byte tiles
+ *                 of 128 rows x 4 blocks: tile (r / 128) * ceil(blocks / 4) +
+ *                 b / 4, byte r % 32 * 16 + r % 128 / 32 * 4 + b % 4.  Blocks
+ *                 behind the last one (up to a whole tile) are written as 0;
+ *                 rows behind the last one are not written.  16-byte aligned. */
+typedef enum { NQ_MXFP4 = 0, NQ_NVFP4 = 1 } nq_mx4_format_t;
+
+/* 0 for a negative size or an unknown format.  The entry points below take up to
+   2^30 columns. */
+size_t nq_mx4_row_bytes(int cols);
+size_t nq_mx4_scale_bytes(int rows, int cols, nq_mx4_format_t fmt);
+/* Quantizes a rows x cols matrix (NQ_F32 or NQ_BF16; rows src_stride elements
+   apart, 0 = cols).  row_scales: [rows], required for NQ_NVFP4, NULL for
+   NQ_MXFP4.  One launch. */
+nq_status_t nq_quantize_rows_mx4(const void* src, nq_dtype_t src_dtype, int src_stride, uint8_t* codes,
+                                 uint8_t* block_scales, float* row_scales, int rows, int cols,
+                                 nq_mx4_format_t fmt, nq_stream_t s);
+/* dst[r][c] = (code * block scale) * row scale, dst rows x cols dense, NQ_F32 or
+   NQ_BF16 (one more rounding).  row_scales may be NULL (no factor). */
+nq_status_t nq_dequantize_rows_mx4(const uint8_t* codes, const uint8_t* block_scales, const float* row_scales,
+                                   void* dst, nq_dtype_t dst_dtype, int rows, int cols, nq_mx4_format_t fmt,
+                                   nq_stream_t s);
+
+/* out[m, n] = epi( sum_k A[m, k] * B[n, k] ): A m x k and B n x k both in the
+ * 4-bit storage above (B "packed", NQ_B_NK), block scales applied inside the
+ * product (tcgen05 kind::mxf4 / kind::mxf4nvf4 with block scaling), fp32 sums.
+ *   epi(acc) = ((acc * alpha) [* row_scale[m]]) [* col_scale[n]] [+ bias[n]]
+ * as in nq_gemm; the NVFP4 row scales of A and B are passed as row_scale and
+ * col_scale.  out: m x n dense, NQ_F32 or NQ_BF16, any m, n, k >= 0 (k = 0: the
+ * sum is 0). */
+typedef struct {
+    int m, n, k;
+    nq_mx4_format_t format;
+    nq_dtype_t out_dtype;   /* NQ_F32 or NQ_BF16 */
+    float alpha;
+    const float* row_scale; /* [m] device, or NULL */
+    const float* col_scale; /* [n] device, or NULL */
+    const float* bias;      /* [n] device, or NULL */
+} nq_gemm_mx4_desc_t;
+nq_status_t nq_gemm_mx4(const nq_gemm_mx4_desc_t* desc, const uint8_t* a_codes, const uint8_t* a_scales,
+                        const uint8_t* b_codes, const uint8_t* b_scales, void* out, nq_stream_t s);
+
+/* ---- RMS norm with the residual's addition and a quantized output -------------
+ * No reference counterpart.  For every row of a rows x cols matrix
+ *   h = x + residual  (rounded to the tensors' type; h = x without residual)
+ *   t = h * weight,  r = 1 / sqrt(mean(h^2) + eps),  y = t * r
+ * in fp32.  The residual stream and the operand of the next linear layer leave
+ * in one launch:
+ *   sum     h, dense, or NULL; may be x or residual itself (then that tensor
+ *           must be dense).  Only with a residual;
+ *   y       y rounded to the tensors' type, dense, or NULL;
+ *   codes   the quantized y, or NULL (then scales is NULL too).
+ * 8-bit output, as nq_quantize_rows defines it (a row's factor r cancels in the
+ * codes): T = max |t|, scales[r] = r T / qmax (1.0 for T = 0), code =
+ * encode(t * (qmax / T)), T at least 2^-110.  A row that holds an infinity or
+ * NaN has a NaN scale.  4-bit output: NQ_MXFP4 of y; NQ_NVFP4 codes and block
+ * scales of t, row scale r A / 2688. */
+typedef struct {
+    int rows, cols;
+    nq_dtype_t dtype;        /* of x, residual, sum, y and gradients: NQ_F32 or NQ_BF16 */
+    nq_dtype_t weight_dtype; /* NQ_F32 or NQ_BF16 */
+    float eps;               /* >= 0 */
+    int x_stride;            /* elements between rows of x; 0 = cols */
+    int residual_stride;     /* elements between rows of residual; 0 = cols */
+} nq_rmsnorm_desc_t;
+
+nq_status_t nq_rmsnorm_quantize(const nq_rmsnorm_desc_t* desc, const void* x, const void* residual,
+                                const void* weight, void* sum, void* y, uint8_t* codes, float* scales,
+                                nq_format_t fmt, nq_stream_t s);
+nq_status_t nq_rmsnorm_quantize_mx4(const nq_rmsnorm_desc_t* desc, const void* x, const void* residual,
+                                    const void* weight, void* sum, void* y, uint8_t* codes,
+                                    uint8_t* block_scales, float* row_scales, nq_mx4_format_t fmt,
+                                    nq_stream_t s);
+/* Gradients of the norm; the rounding of the codes counts as the identity.
+ *   h        the normalized rows: `sum`, or x where there was no residual
+ *            (desc->x_stride apart);
+ *   grad_y   gradient of y, dense;
+ *   grad_sum gradient of the residual stream behind the addition, dense, or NULL;
+ *   grad_x   grad_sum + r g - h r^3 mean(g h), g = grad_y * weight: the gradient
+ *            of x and of residual, dense, or NULL to skip; may be grad_sum
+ *            itself;
+ *   grad_weight  fp32 [cols], sum over rows of grad_y * h * r (overwritten, in a
+ *            fixed order), or NULL to skip. */
+nq_status_t nq_rmsnorm_backward(const nq_rmsnorm_desc_t* desc, const void* h, const void* weight,
+                                const void* grad_y, const void* grad_sum, void* grad_x, float* grad_weight,
+                                nq_stream_t s);
+
 #ifdef __cplusplus
 }
 #endif

@@ -19,6 +19,7 @@ lib = C.CDLL(LIB_PATH)
 E4M3, E5M2, INT8 = 0, 1, 2
 F32, BF16, S32, S8 = 0, 1, 2, 3
 B_KN, B_NK = 0, 1
+MXFP4, NVFP4 = 0, 1
 
 _p, _sz, _f, _i, _u32p = C.c_void_p, C.c_size_t, C.c_float, C.c_int, C.POINTER(C.c_uint32)
 
@@ -48,6 +49,16 @@ class AllreduceDesc(C.Structure):
                 ("peer_partial", C.c_void_p * MAX_TP), ("peer_out", C.c_void_p * MAX_TP),
                 ("peer_done", C.c_void_p * MAX_TP),
                 ("done", C.c_void_p), ("done_target", C.c_uint32)]
+
+
+class GemmMx4Desc(C.Structure):
+    _fields_ = [("m", C.c_int), ("n", C.c_int), ("k", C.c_int), ("format", C.c_int), ("out_dtype", C.c_int),
+                ("alpha", C.c_float), ("row_scale", C.c_void_p), ("col_scale", C.c_void_p), ("bias", C.c_void_p)]
+
+
+class RmsnormDesc(C.Structure):
+    _fields_ = [("rows", C.c_int), ("cols", C.c_int), ("dtype", C.c_int), ("weight_dtype", C.c_int),
+                ("eps", C.c_float), ("x_stride", C.c_int), ("residual_stride", C.c_int)]
 
 
 _SIGS = {
@@ -86,6 +97,12 @@ _SIGS = {
     "nq_set_peer_wait_limit": [C.c_uint64],
     "nq_mixed_precision_matmul": [_p, _p, _p, _p, _i, _i, _i, _p],
     "nq_fp8_gemm_backward": [_p, _i, _p, _p, _p, _p, _i, _i, _i, _f, _f, _f, _p],
+    "nq_quantize_rows_mx4": [_p, _i, _i, _p, _p, _p, _i, _i, _i, _p],
+    "nq_dequantize_rows_mx4": [_p, _p, _p, _p, _i, _i, _i, _i, _p],
+    "nq_gemm_mx4": [C.POINTER(GemmMx4Desc), _p, _p, _p, _p, _p, _p],
+    "nq_rmsnorm_quantize": [C.POINTER(RmsnormDesc), _p, _p, _p, _p, _p, _p, _p, _i, _p],
+    "nq_rmsnorm_quantize_mx4": [C.POINTER(RmsnormDesc), _p, _p, _p, _p, _p, _p, _p, _p, _i, _p],
+    "nq_rmsnorm_backward": [C.POINTER(RmsnormDesc), _p, _p, _p, _p, _p, _p, _p],
 }
 
 lib.nq_status_string.restype = C.c_char_p
@@ -104,6 +121,12 @@ peer_wait_limit = lib.nq_peer_wait_limit
 lib.nq_allreduce_done_per_job.restype = C.c_int
 lib.nq_allreduce_done_per_job.argtypes = [_i, _i, _i]
 allreduce_done_per_job = lib.nq_allreduce_done_per_job
+lib.nq_mx4_row_bytes.restype = C.c_size_t
+lib.nq_mx4_row_bytes.argtypes = [_i]
+mx4_row_bytes = lib.nq_mx4_row_bytes
+lib.nq_mx4_scale_bytes.restype = C.c_size_t
+lib.nq_mx4_scale_bytes.argtypes = [_i, _i, _i]
+mx4_scale_bytes = lib.nq_mx4_scale_bytes
 
 
 def _wrap(name, argtypes):
@@ -129,7 +152,8 @@ for _n, _a in _SIGS.items():
 
 def exported_symbols():
     return sorted(list(_SIGS) + ["nq_status_string", "nq_last_error", "nq_version", "nq_fp8_gemm_workspace_size",
-                                 "nq_gemm_allreduce_counters", "nq_allreduce_done_per_job", "nq_peer_wait_limit"])
+                                 "nq_gemm_allreduce_counters", "nq_allreduce_done_per_job", "nq_peer_wait_limit",
+                                 "nq_mx4_row_bytes", "nq_mx4_scale_bytes"])
 
 
 EPI_NONE, EPI_SWIGLU = 0, 1
@@ -140,6 +164,14 @@ def make_desc(m, n, k, a_format=E4M3, b_format=E4M3, b_layout=B_KN, out_dtype=BF
               row_scale=0, col_scale=0, bias=0, epilogue=EPI_NONE) -> GemmDesc:
     return GemmDesc(m, n, k, a_format, b_format, b_layout, out_dtype, alpha, row_scale or None,
                     col_scale or None, bias or None, epilogue)
+
+
+def make_mx4_desc(m, n, k, format=NVFP4, out_dtype=BF16, alpha=1.0, row_scale=0, col_scale=0, bias=0) -> GemmMx4Desc:
+    return GemmMx4Desc(m, n, k, format, out_dtype, alpha, row_scale or None, col_scale or None, bias or None)
+
+
+def make_rmsnorm_desc(rows, cols, dtype=BF16, weight_dtype=BF16, eps=1e-5, x_stride=0, residual_stride=0) -> RmsnormDesc:
+    return RmsnormDesc(rows, cols, dtype, weight_dtype, eps, x_stride, residual_stride)
 
 
 def device_error_flags(clear: bool = True) -> int:

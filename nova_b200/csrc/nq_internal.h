@@ -72,6 +72,10 @@ uint32_t* device_error_word();
 uint64_t peer_wait_limit_ns();
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+// Aligned to an element of NQ_F32 or NQ_BF16.
+inline bool aligned_to(const void* p, nq_dtype_t dt) {
+    return (reinterpret_cast<uintptr_t>(p) & (dt == NQ_BF16 ? 1u : 3u)) == 0;
+}
 
 // Runs init() once per device for one call site (e.g. a kernel's shared-memory
 // opt-in, a per-device function attribute).  Bit `device` of `done` is read
