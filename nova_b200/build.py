@@ -19,8 +19,8 @@ ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libnova_q.so")
-SOURCES = ["runtime.cu", "elementwise.cu", "reduce.cu", "gemm.cu", "mx4.cu", "norm.cu"]
-HEADERS = ["nq_internal.h", "ptx.cuh", "codec.cuh", "mx4.cuh"]
+SOURCES = ["runtime.cu", "elementwise.cu", "reduce.cu", "gemm.cu", "mx4.cu", "mx4_gemm.cu", "norm.cu"]
+HEADERS = ["nq_internal.h", "ptx.cuh", "codec.cuh", "mx4.cuh", "tmap.h"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-std=c++17", "-O3", "-lineinfo", "-Xcompiler", "-fPIC", "-Xcompiler", "-O2"] + ARCH
 

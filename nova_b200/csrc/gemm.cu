@@ -31,6 +31,7 @@
 #include "codec.cuh"
 #include "nq_internal.h"
 #include "ptx.cuh"
+#include "tmap.h"
 
 namespace nq {
 namespace {
@@ -460,21 +461,6 @@ __device__ __forceinline__ void tile_coords(int tile, int m_tiles, int n_tiles, 
     mb = band * P_BAND + local % rows;
     nb = local / rows;
 }
-// Spins (bounded) until *flag >= want, reading with acquire semantics.
-__device__ __forceinline__ bool wait_flag_geq(const uint32_t* flag, uint32_t want, uint32_t* err) {
-    const uint64_t t0 = globaltimer();
-    while (true) {
-        uint32_t v;
-        asm volatile("ld.global.acquire.gpu.u32 %0, [%1];" : "=r"(v) : "l"(flag) : "memory");
-        if (v >= want) return true;
-        if (globaltimer() - t0 > kWaitLimitNs) {
-            if (err) atomicOr(err, kErrWaitTimeout);
-            return false;
-        }
-        __nanosleep(64);
-    }
-}
-
 // Spins (bounded by `limit` ns) until the system-scope counter at p has
 // reached `want`.  The all-reduce counters only grow and are compared modulo
 // 2^32 (the signed difference), so a counter and a target that both wrapped
@@ -1744,50 +1730,6 @@ __global__ void __launch_bounds__(256) k_gemm_simt(const uint8_t* __restrict__ a
 }
 
 // ---------------- host side ----------------
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-nq_status_t get_encode_fn(EncodeTiledFn* fn) {
-    static std::atomic<EncodeTiledFn> cached{nullptr};
-    static std::mutex mu;
-    EncodeTiledFn f = cached.load(std::memory_order_acquire);
-    if (!f) {
-        std::lock_guard<std::mutex> lk(mu);
-        f = cached.load(std::memory_order_relaxed);
-        if (!f) {
-            void* p = nullptr;
-            cudaDriverEntryPointQueryResult q;
-            cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q);
-            if (e != cudaSuccess || q != cudaDriverEntryPointSuccess || !p)
-                return fail(NQ_ERROR_CUDA, "cuTensorMapEncodeTiled entry point not found");
-            f = reinterpret_cast<EncodeTiledFn>(p);
-            cached.store(f, std::memory_order_release);
-        }
-    }
-    *fn = f;
-    return NQ_SUCCESS;
-}
-
-// 2-D uint8 tensor map: inner extent `inner`, `outer` rows of `ld` bytes,
-// box {box_inner, box_outer}, 128-byte swizzle, zero fill out of bounds.
-nq_status_t make_map(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer, uint64_t ld,
-                     uint32_t box_inner, uint32_t box_outer,
-                     CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B) {
-    EncodeTiledFn fn;
-    nq_status_t st = get_encode_fn(&fn);
-    if (st != NQ_SUCCESS) return st;
-    cuuint64_t dims[2] = {inner, outer};
-    cuuint64_t strides[1] = {ld};
-    cuuint32_t box[2] = {box_inner, box_outer};
-    cuuint32_t estr[2] = {1, 1};
-    CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
-                    CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS) return fail(NQ_ERROR_CUDA, "cuTensorMapEncodeTiled failed (" + std::to_string(int(r)) + ")");
-    return NQ_SUCCESS;
-}
-
 // The shared-memory opt-in is a per-device function attribute.
 template <class F>
 nq_status_t ensure_smem_attr(F kern, int bytes, int device, std::atomic<uint64_t>* flags) {

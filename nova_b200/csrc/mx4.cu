@@ -1,5 +1,4 @@
-// mx4.cu -- microscaled 4-bit formats: quantize, dequantize and the product of
-// two quantized operands.
+// mx4.cu -- microscaled 4-bit formats: quantize and dequantize.
 #include <algorithm>
 #include <string>
 
@@ -85,48 +84,6 @@ __global__ void __launch_bounds__(kThreads) k_mx4_dequant(const uint8_t* __restr
             store_raw8<T, VEC>(dst + static_cast<size_t>(row) * cols, v, cols, pack8<T>(f));
         }
     }
-}
-
-struct MxEpi {
-    void* out;
-    int out_bf16;
-    float alpha;
-    const float* row_scale;
-    const float* col_scale;
-    const float* bias;
-};
-
-// One thread per output, 8 columns a step.
-template <int F>
-__global__ void __launch_bounds__(256) k_mx4_gemm_simt(const uint8_t* __restrict__ a, const uint8_t* __restrict__ as,
-                                                       const uint8_t* __restrict__ b, const uint8_t* __restrict__ bs, int M,
-                                                       int N, int K, MxEpi ep) {
-    const int n = blockIdx.x * 16 + (threadIdx.x & 15), m = blockIdx.y * 16 + (threadIdx.x >> 4);
-    if (m >= M || n >= N) return;
-    constexpr int L = Mx4Traits<F>::block_lanes;
-    const int words = mx4_words(K, Mx4Traits<F>::block);
-    const uint32_t* ca = reinterpret_cast<const uint32_t*>(a + m * mx4_pitch(K));
-    const uint32_t* cb = reinterpret_cast<const uint32_t*>(b + n * mx4_pitch(K));
-    float acc = 0.0f;
-    for (int v = 0; v < (K + 7) / 8; ++v) {
-        float fa[8], fb[8];
-        e2m1_decode8(ca[v], fa);
-        e2m1_decode8(cb[v], fb);
-        float d = 0.0f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) d = __fmaf_rn(fa[e], fb[e], d);
-        const int blk = v / L;
-        const float s = mx4_scale_value(F, as[mx4_scale_offset(m, blk / 4, words) + blk % 4]) *
-                        mx4_scale_value(F, bs[mx4_scale_offset(n, blk / 4, words) + blk % 4]);
-        acc = __fmaf_rn(d, s, acc);
-    }
-    float v = __fmul_rn(acc, ep.alpha);
-    if (ep.row_scale) v = __fmul_rn(v, ep.row_scale[m]);
-    if (ep.col_scale) v = __fmul_rn(v, ep.col_scale[n]);
-    if (ep.bias) v = __fadd_rn(v, ep.bias[n]);
-    const size_t at = static_cast<size_t>(m) * N + n;
-    if (ep.out_bf16) static_cast<uint16_t*>(ep.out)[at] = static_cast<uint16_t>(f32x2_to_bf16x2(v, 0.0f));
-    else static_cast<float*>(ep.out)[at] = v;
 }
 
 // ---- host side -------------------------------------------------------------------
@@ -217,33 +174,6 @@ nq_status_t nq_dequantize_rows_mx4(const uint8_t* codes, const uint8_t* block_sc
     }
     if (dst_dtype == NQ_F32) return vec ? go(k_mx4_dequant<float, kNVFP4, true>, f) : go(k_mx4_dequant<float, kNVFP4, false>, f);
     return vec ? go(k_mx4_dequant<uint16_t, kNVFP4, true>, h) : go(k_mx4_dequant<uint16_t, kNVFP4, false>, h);
-}
-
-nq_status_t nq_gemm_mx4(const nq_gemm_mx4_desc_t* d, const uint8_t* a_codes, const uint8_t* a_scales, const uint8_t* b_codes,
-                        const uint8_t* b_scales, void* out, nq_stream_t s) {
-    const char* who = "nq_gemm_mx4";
-    if (!d) return nq::bad(who, "null descriptor");
-    nq_status_t st = nq::check_matrix(who, d->m, d->k, d->format, d->out_dtype);
-    if (st != NQ_SUCCESS) return st;
-    if (d->n < 0) return nq::bad(who, "negative size");
-    if (d->m == 0 || d->n == 0) return NQ_SUCCESS;
-    if (!out || (d->k > 0 && (!a_codes || !a_scales || !b_codes || !b_scales))) return nq::bad(who, "null pointer");
-    if (!nq::aligned16(a_codes) || !nq::aligned16(a_scales) || !nq::aligned16(b_codes) || !nq::aligned16(b_scales))
-        return nq::bad(who, "codes and block scales must be 16-byte aligned");
-    if (!nq::aligned_to(out, d->out_dtype) || !nq::aligned_to(d->row_scale, NQ_F32) || !nq::aligned_to(d->col_scale, NQ_F32) ||
-        !nq::aligned_to(d->bias, NQ_F32))
-        return nq::bad(who, "a pointer is not aligned to its type");
-    nq::DeviceInfo di;
-    st = nq::current_device(&di);
-    if (st != NQ_SUCCESS) return st;
-    const nq::MxEpi ep{out, d->out_dtype == NQ_BF16, d->alpha, d->row_scale, d->col_scale, d->bias};
-    const dim3 grid((d->n + 15) / 16, (d->m + 15) / 16);
-    if (d->format == NQ_MXFP4)
-        nq::k_mx4_gemm_simt<nq::dev::kMXFP4><<<grid, 256, 0, s>>>(a_codes, a_scales, b_codes, b_scales, d->m, d->n, d->k, ep);
-    else
-        nq::k_mx4_gemm_simt<nq::dev::kNVFP4><<<grid, 256, 0, s>>>(a_codes, a_scales, b_codes, b_scales, d->m, d->n, d->k, ep);
-    NQ_LAUNCH_CHECK(who);
-    return NQ_SUCCESS;
 }
 
 }  // extern "C"

@@ -81,6 +81,21 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, uint32
     }
 }
 
+// Spins (bounded) until *flag >= want, reading with acquire semantics.
+__device__ __forceinline__ bool wait_flag_geq(const uint32_t* flag, uint32_t want, uint32_t* err) {
+    const uint64_t t0 = globaltimer();
+    while (true) {
+        uint32_t v;
+        asm volatile("ld.global.acquire.gpu.u32 %0, [%1];" : "=r"(v) : "l"(flag) : "memory");
+        if (v >= want) return true;
+        if (globaltimer() - t0 > kWaitLimitNs) {
+            if (err) atomicOr(err, kErrWaitTimeout);
+            return false;
+        }
+        __nanosleep(64);
+    }
+}
+
 // Cluster-scope release add / acquire load on a shared::cluster address (mapa).
 __device__ __forceinline__ void red_add_release_cluster(uint32_t cluster_saddr, uint32_t v) {
     asm volatile("red.release.cluster.shared::cluster.add.u32 [%0], %1;" ::"r"(cluster_saddr), "r"(v) : "memory");
@@ -335,6 +350,57 @@ __device__ __forceinline__ void tc_commit_pair_mc(uint64_t* bar, uint16_t cta_ma
         : "memory");
 }
 
+// Block-scaled 4-bit MMA: D (+)= (A * SFA) * (B * SFB), E2M1 operands, K = 64.
+// MX: kind::mxf4, one E8M0 scale per 32 columns; else kind::mxf4nvf4, one E4M3
+// scale per 16.  The scales lie in tensor memory, row r of an operand in lane
+// r % 32 (repeated in the four lane quarters), column r / 32, one byte per block.
+template <bool MX>
+__device__ __forceinline__ void mma_mx4(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t sfa,
+                                        uint32_t sfb, uint32_t accumulate) {
+    if (MX)
+        asm volatile(
+            "{\n\t.reg .pred P;\n\t"
+            "setp.ne.b32 P, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], P;\n\t}" ::"r"(d_tmem),
+            "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred P;\n\t"
+            "setp.ne.b32 P, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], P;\n\t}" ::"r"(d_tmem),
+            "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+            : "memory");
+}
+template <bool MX>
+__device__ __forceinline__ void mma_mx4_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t sfa,
+                                             uint32_t sfb, uint32_t accumulate) {
+    if (MX)
+        asm volatile(
+            "{\n\t.reg .pred P;\n\t"
+            "setp.ne.b32 P, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], P;\n\t}" ::"r"(d_tmem),
+            "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred P;\n\t"
+            "setp.ne.b32 P, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], P;\n\t}" ::"r"(d_tmem),
+            "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+            : "memory");
+}
+// One 512-byte scale tile (32 rows of 16 bytes, unswizzled) from shared memory
+// to 4 tensor memory columns, repeated in the four lane quarters; the pair form
+// copies in both CTAs, each from its own shared memory.  Ordered before the
+// MMAs that the same thread issues after it.
+__device__ __forceinline__ void tmem_cp_scales(uint32_t taddr, uint64_t desc) {
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+__device__ __forceinline__ void tmem_cp_scales_pair(uint32_t taddr, uint64_t desc) {
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+
 // 32 lanes x 32 bits, 32 consecutive columns: r[j] = TMEM[lane][col + j].
 __device__ __forceinline__ void tmem_ld_32x32b_x32(uint32_t taddr, uint32_t (&r)[32]) {
     asm volatile(
@@ -398,6 +464,25 @@ __device__ __forceinline__ uint64_t smem_desc_sw64(uint32_t saddr, uint32_t lbo_
     d |= 4ull << 61;
     return d;
 }
+
+// Unswizzled rows of 16 bytes, 8-row groups 128 bytes apart (scale tiles).
+__device__ __forceinline__ uint64_t smem_desc_rows16(uint32_t saddr) {
+    uint64_t d = 0;
+    d |= static_cast<uint64_t>((saddr >> 4) & 0x3FFFu);
+    d |= static_cast<uint64_t>(1) << 16;
+    d |= static_cast<uint64_t>(128 >> 4) << 32;
+    d |= 1ull << 46;
+    return d;
+}
+
+// Instruction descriptor of the block-scaled 4-bit MMAs:
+//   [4,6) B scale id, [7,10) A format, [10,12) B format (1 = E2M1), [17,23) N >> 3,
+//   [23] scale type (0 = E4M3, 1 = E8M0), [27,29) M >> 7, [29,31) A scale id.
+// The scale ids pick the bytes of a scale word that an MMA uses (mxf4: 0 or 2).
+__host__ __device__ constexpr uint32_t make_idesc_mx4(bool mx, uint32_t m, uint32_t n) {
+    return (1u << 7) | (1u << 10) | ((n >> 3) << 17) | ((mx ? 1u : 0u) << 23) | ((m >> 7) << 27);
+}
+__host__ __device__ constexpr uint32_t idesc_scale_ids(uint32_t id) { return (id << 4) | (id << 29); }
 
 // Instruction descriptor of tcgen05.mma kind::f8f6f4 / kind::i8:
 //   [4,6) D format (1 = f32, 2 = s32), [7,10) A format, [10,13) B format,
