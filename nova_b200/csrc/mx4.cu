@@ -22,17 +22,29 @@ __device__ __forceinline__ uint32_t block_umax(uint32_t m, int parity) {
     return __reduce_max_sync(0xffffffffu, l < (blockDim.x >> 5) ? s_max[parity][l] : 0u);
 }
 
-// One block per row; NVFP4 reads the row twice (its maximum first).
+template <bool VEC>
+__device__ __forceinline__ uint8_t* warp_buf() {
+    if constexpr (VEC) {
+        return nullptr;
+    } else {
+        __shared__ uint4 s_buf[32 * kWarpBuf / 16];
+        return reinterpret_cast<uint8_t*>(s_buf) + (threadIdx.x >> 5) * kWarpBuf;
+    }
+}
+
+// One block per row; NVFP4 reads the row twice (its maximum first).  For rows too wide for k_mx4_quant.
 template <class In, int F, bool VEC>
-__global__ void __launch_bounds__(kThreads) k_mx4_quant(const In* __restrict__ src, size_t ld, uint8_t* __restrict__ codes,
-                                                        uint8_t* __restrict__ bscales, float* __restrict__ rscales, int rows,
-                                                        int cols) {
+__global__ void __launch_bounds__(kThreads) k_mx4_quant_wide(const In* __restrict__ src, size_t ld, uint8_t* __restrict__ codes,
+                                                             uint8_t* __restrict__ bscales, float* __restrict__ rscales,
+                                                             int rows, int cols) {
     pdl_launch_dependents();
     pdl_wait();
+    uint8_t* buf = warp_buf<VEC>();
     const int nvec = (cols + 7) / 8;
     const int words = mx4_words(cols, Mx4Traits<F>::block);
     const int pitch_words = static_cast<int>(mx4_pitch(cols) / 4);
     const int nstep = words * Mx4Traits<F>::word_lanes;
+    const int lane = lane_of();
     int parity = 0;
     for (long long rl = blockIdx.x; rl < rows; rl += gridDim.x, parity ^= 1) {
         const int row = static_cast<int>(rl);
@@ -41,9 +53,9 @@ __global__ void __launch_bounds__(kThreads) k_mx4_quant(const In* __restrict__ s
         bool ok = true;
         if (F == kNVFP4) {
             uint32_t m = 0;
-            for (int v = threadIdx.x; v < nvec; v += kThreads) {
+            for (int v = threadIdx.x; v - lane < nvec; v += kThreads) {
                 float f[8];
-                unpack8<In>(load_raw8<In, VEC>(x, v, cols), f);
+                unpack8<In>(load_vec<In, VEC>(x, v, cols, buf), f);
                 m = max(m, amax_bits8(f));
             }
             m = block_umax(m, parity);
@@ -51,9 +63,9 @@ __global__ void __launch_bounds__(kThreads) k_mx4_quant(const In* __restrict__ s
             level = nv_row_level(m);
             if (threadIdx.x == 0) rscales[row] = nv_row_scale(m, level);
         }
-        for (int v = threadIdx.x; v - static_cast<int>(threadIdx.x & 31) < nstep; v += kThreads) {
+        for (int v = threadIdx.x; v - lane < nstep; v += kThreads) {
             float f[8];
-            unpack8<In>(load_raw8<In, VEC>(x, v, cols), f);
+            unpack8<In>(load_vec<In, VEC>(x, v, cols, buf), f);
             uint32_t byte;
             const uint32_t c = mx4_encode<F>(f, level, ok, &byte);
             mx4_store<F>(codes + row * mx4_pitch(cols), bscales, row, v, pitch_words, words, c, byte);
@@ -61,27 +73,88 @@ __global__ void __launch_bounds__(kThreads) k_mx4_quant(const In* __restrict__ s
     }
 }
 
+// Rows held in registers, NV vectors of 8 columns a thread, by one warp (WARP) or
+// one block; each row is read once.
+template <class In, int F, bool VEC, int NV, bool WARP>
+__global__ void __launch_bounds__(WARP ? 256 : 1024) k_mx4_quant(const In* __restrict__ src, size_t ld,
+                                                                 uint8_t* __restrict__ codes, uint8_t* __restrict__ bscales,
+                                                                 float* __restrict__ rscales, int rows, int cols) {
+    pdl_launch_dependents();
+    uint8_t* buf = warp_buf<VEC>();
+    const int words = mx4_words(cols, Mx4Traits<F>::block);
+    const int pitch_words = static_cast<int>(mx4_pitch(cols) / 4);
+    const int width = WARP ? 32 : blockDim.x;
+    const int t0 = WARP ? lane_of() : threadIdx.x;
+    const int per = WARP ? blockDim.x >> 5 : 1;
+    pdl_wait();
+    int parity = 0;
+    for (long long rl = static_cast<long long>(blockIdx.x) * per + (WARP ? threadIdx.x >> 5 : 0); rl < rows;
+         rl += static_cast<long long>(gridDim.x) * per, parity ^= 1) {
+        const int row = static_cast<int>(rl);
+        Raw8<In> x[NV];
+        load_vecs<In, VEC, NV>(x, src + row * ld, t0, width, cols, buf);
+        float level = 0.0f;
+        bool ok = true;
+        if (F == kNVFP4) {
+            uint32_t m = 0;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                float f[8];
+                unpack8<In>(x[i], f);
+                m = max(m, amax_bits8(f));
+            }
+            m = WARP ? __reduce_max_sync(0xffffffffu, m) : block_umax(m, parity);
+            ok = m < kInfBits;
+            level = nv_row_level(m);
+            if (t0 == 0) rscales[row] = nv_row_scale(m, level);
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            float f[8];
+            unpack8<In>(x[i], f);
+            uint32_t byte;
+            const uint32_t c = mx4_encode<F>(f, level, ok, &byte);
+            mx4_store<F>(codes + row * mx4_pitch(cols), bscales, row, t0 + i * width, pitch_words, words, c, byte);
+        }
+    }
+}
+
+// `width` threads a row, four vectors a thread in flight.
 template <class T, int F, bool VEC>
 __global__ void __launch_bounds__(kThreads) k_mx4_dequant(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ bscales,
                                                           const float* __restrict__ rscales, T* __restrict__ dst, int rows,
-                                                          int cols) {
+                                                          int cols, int width) {
     pdl_launch_dependents();
-    pdl_wait();
+    uint8_t* buf = warp_buf<VEC>();
     constexpr int L = Mx4Traits<F>::block_lanes;
     const int nvec = (cols + 7) / 8;
     const int words = mx4_words(cols, Mx4Traits<F>::block);
-    for (long long rl = blockIdx.x; rl < rows; rl += gridDim.x) {
+    const int t0 = threadIdx.x % width;
+    const int per = kThreads / width;
+    pdl_wait();
+    for (long long rl = static_cast<long long>(blockIdx.x) * per + threadIdx.x / width; rl < rows;
+         rl += static_cast<long long>(gridDim.x) * per) {
         const int row = static_cast<int>(rl);
         const float g = rscales ? __ldg(rscales + row) : 1.0f;
         const uint32_t* code = reinterpret_cast<const uint32_t*>(codes + row * mx4_pitch(cols));
-        for (int v = threadIdx.x; v < nvec; v += kThreads) {
-            const int b = v / L;
-            const float s = mx4_scale_value(F, __ldg(bscales + mx4_scale_offset(row, b / 4, words) + b % 4));
-            float f[8];
-            e2m1_decode8(__ldg(code + v), f);
+        T* out = dst + static_cast<size_t>(row) * cols;
+        for (int v0 = t0; v0 - lane_of() < nvec; v0 += 4 * width) {
+            uint32_t c[4], s[4];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) f[e] = __fmul_rn(__fmul_rn(f[e], s), g);
-            store_raw8<T, VEC>(dst + static_cast<size_t>(row) * cols, v, cols, pack8<T>(f));
+            for (int i = 0; i < 4; ++i) {
+                const int v = v0 + i * width, b = v / L;
+                c[i] = v < nvec ? __ldg(code + v) : 0u;
+                s[i] = v < nvec ? __ldg(bscales + mx4_scale_offset(row, b / 4, words) + b % 4) : 0u;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float f[8];
+                e2m1_decode8(c[i], f);
+                const float sv = mx4_scale_value(F, s[i]);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) f[e] = __fmul_rn(__fmul_rn(f[e], sv), g);
+                store_vec<T, VEC>(out, v0 + i * width, cols, pack8<T>(f), buf);
+            }
         }
     }
 }
@@ -97,6 +170,58 @@ nq_status_t check_matrix(const char* who, int rows, int cols, nq_mx4_format_t fm
     if (fmt != NQ_MXFP4 && fmt != NQ_NVFP4) return bad(who, "format");
     if (dt != NQ_F32 && dt != NQ_BF16) return bad(who, "dtype must be NQ_F32 or NQ_BF16");
     return NQ_SUCCESS;
+}
+
+struct QuantArgs {
+    size_t ld;
+    uint8_t* codes;
+    uint8_t* bscales;
+    float* rscales;
+    int rows, cols;
+};
+
+template <class In, int F, bool VEC, int NV, bool WARP>
+nq_status_t launch_quant(const In* src, const QuantArgs& a, int threads, const DeviceInfo& di, cudaStream_t s) {
+    auto kern = k_mx4_quant<In, F, VEC, NV, WARP>;
+    int per_sm = 0;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, threads, 0) != cudaSuccess || per_sm < 1) {
+        cudaGetLastError();
+        per_sm = 1;
+    }
+    const long long blocks = WARP ? (static_cast<long long>(a.rows) + threads / 32 - 1) / (threads / 32) : a.rows;
+    const int grid = static_cast<int>(std::min<long long>(blocks, static_cast<long long>(di.sm_count) * per_sm));
+    return cuda_status(launch_pdl(kern, dim3(grid), dim3(threads), 0, s, src, a.ld, a.codes, a.bscales, a.rscales, a.rows, a.cols),
+                       "nq_quantize_rows_mx4");
+}
+
+template <class In, int F, bool VEC>
+nq_status_t quant_impl(const void* p, const QuantArgs& a, const DeviceInfo& di, cudaStream_t s) {
+    constexpr int NVMAX = sizeof(In) == 2 ? 4 : 2;  // 64 bytes a thread
+    const In* src = static_cast<const In*>(p);
+    const int nvec = mx4_words(a.cols, Mx4Traits<F>::block) * Mx4Traits<F>::word_lanes;  // whole scale words
+    if (nvec <= 32) return launch_quant<In, F, VEC, 1, true>(src, a, 256, di, s);
+    if (nvec <= 32 * NVMAX) return launch_quant<In, F, VEC, NVMAX, true>(src, a, 256, di, s);
+    if (a.rows < 2 * di.sm_count && nvec <= 1024) return launch_quant<In, F, VEC, 1, false>(src, a, (nvec + 31) / 32 * 32, di, s);
+    const int threads = ((nvec + NVMAX - 1) / NVMAX + 31) / 32 * 32;
+    if (threads <= 1024) return launch_quant<In, F, VEC, NVMAX, false>(src, a, threads, di, s);
+    const int grid = static_cast<int>(std::min<long long>(a.rows, static_cast<long long>(di.sm_count) * 8));
+    return cuda_status(launch_pdl(k_mx4_quant_wide<In, F, VEC>, dim3(grid), dim3(kThreads), 0, s, src, a.ld, a.codes, a.bscales,
+                                  a.rscales, a.rows, a.cols),
+                       "nq_quantize_rows_mx4 (wide)");
+}
+
+template <class T, int F>
+nq_status_t dequant_impl(const uint8_t* codes, const uint8_t* bscales, const float* rscales, void* dst, int rows, int cols,
+                         bool vec, const DeviceInfo& di, cudaStream_t s) {
+    const int nvec = (cols + 7) / 8;
+    int width = 32;
+    while (width < kThreads && 4 * width < nvec) width *= 2;
+    const long long blocks = (static_cast<long long>(rows) + kThreads / width - 1) / (kThreads / width);
+    const int grid = static_cast<int>(std::min<long long>(blocks, static_cast<long long>(di.sm_count) * 8));
+    auto kern = vec ? k_mx4_dequant<T, F, true> : k_mx4_dequant<T, F, false>;
+    return cuda_status(launch_pdl(kern, dim3(grid), dim3(kThreads), 0, s, codes, bscales, rscales, static_cast<T*>(dst), rows, cols,
+                                  width),
+                       "nq_dequantize_rows_mx4");
 }
 
 }  // namespace
@@ -129,21 +254,14 @@ nq_status_t nq_quantize_rows_mx4(const void* src, nq_dtype_t src_dtype, int src_
     if (st != NQ_SUCCESS) return st;
     const size_t ld = src_stride ? src_stride : cols;
     const bool vec = cols % 8 == 0 && ld * (src_dtype == NQ_BF16 ? 2 : 4) % 16 == 0 && nq::aligned16(src);
-    const int grid = static_cast<int>(std::min<long long>(rows, static_cast<long long>(di.sm_count) * 8));
-    auto go = [&](auto kern, const auto* typed) {
-        return nq::cuda_status(nq::launch_pdl(kern, dim3(grid), dim3(nq::kThreads), 0, s, typed, ld, codes, block_scales,
-                                              row_scales, rows, cols),
-                               who);
-    };
+    const nq::QuantArgs a{ld, codes, block_scales, row_scales, rows, cols};
     using namespace nq;
-    const float* f = static_cast<const float*>(src);
-    const uint16_t* h = static_cast<const uint16_t*>(src);
     if (fmt == NQ_MXFP4) {
-        if (src_dtype == NQ_F32) return vec ? go(k_mx4_quant<float, kMXFP4, true>, f) : go(k_mx4_quant<float, kMXFP4, false>, f);
-        return vec ? go(k_mx4_quant<uint16_t, kMXFP4, true>, h) : go(k_mx4_quant<uint16_t, kMXFP4, false>, h);
+        if (src_dtype == NQ_F32) return vec ? quant_impl<float, kMXFP4, true>(src, a, di, s) : quant_impl<float, kMXFP4, false>(src, a, di, s);
+        return vec ? quant_impl<uint16_t, kMXFP4, true>(src, a, di, s) : quant_impl<uint16_t, kMXFP4, false>(src, a, di, s);
     }
-    if (src_dtype == NQ_F32) return vec ? go(k_mx4_quant<float, kNVFP4, true>, f) : go(k_mx4_quant<float, kNVFP4, false>, f);
-    return vec ? go(k_mx4_quant<uint16_t, kNVFP4, true>, h) : go(k_mx4_quant<uint16_t, kNVFP4, false>, h);
+    if (src_dtype == NQ_F32) return vec ? quant_impl<float, kNVFP4, true>(src, a, di, s) : quant_impl<float, kNVFP4, false>(src, a, di, s);
+    return vec ? quant_impl<uint16_t, kNVFP4, true>(src, a, di, s) : quant_impl<uint16_t, kNVFP4, false>(src, a, di, s);
 }
 
 nq_status_t nq_dequantize_rows_mx4(const uint8_t* codes, const uint8_t* block_scales, const float* row_scales, void* dst,
@@ -159,21 +277,12 @@ nq_status_t nq_dequantize_rows_mx4(const uint8_t* codes, const uint8_t* block_sc
     st = nq::current_device(&di);
     if (st != NQ_SUCCESS) return st;
     const bool vec = cols % 8 == 0 && nq::aligned16(dst);
-    const int grid = static_cast<int>(std::min<long long>(rows, static_cast<long long>(di.sm_count) * 8));
-    auto go = [&](auto kern, auto* typed) {
-        return nq::cuda_status(nq::launch_pdl(kern, dim3(grid), dim3(nq::kThreads), 0, s, codes, block_scales, row_scales,
-                                              typed, rows, cols),
-                               who);
-    };
     using namespace nq;
-    float* f = static_cast<float*>(dst);
-    uint16_t* h = static_cast<uint16_t*>(dst);
-    if (fmt == NQ_MXFP4) {
-        if (dst_dtype == NQ_F32) return vec ? go(k_mx4_dequant<float, kMXFP4, true>, f) : go(k_mx4_dequant<float, kMXFP4, false>, f);
-        return vec ? go(k_mx4_dequant<uint16_t, kMXFP4, true>, h) : go(k_mx4_dequant<uint16_t, kMXFP4, false>, h);
-    }
-    if (dst_dtype == NQ_F32) return vec ? go(k_mx4_dequant<float, kNVFP4, true>, f) : go(k_mx4_dequant<float, kNVFP4, false>, f);
-    return vec ? go(k_mx4_dequant<uint16_t, kNVFP4, true>, h) : go(k_mx4_dequant<uint16_t, kNVFP4, false>, h);
+    if (fmt == NQ_MXFP4)
+        return dst_dtype == NQ_F32 ? dequant_impl<float, kMXFP4>(codes, block_scales, row_scales, dst, rows, cols, vec, di, s)
+                                   : dequant_impl<uint16_t, kMXFP4>(codes, block_scales, row_scales, dst, rows, cols, vec, di, s);
+    return dst_dtype == NQ_F32 ? dequant_impl<float, kNVFP4>(codes, block_scales, row_scales, dst, rows, cols, vec, di, s)
+                               : dequant_impl<uint16_t, kNVFP4>(codes, block_scales, row_scales, dst, rows, cols, vec, di, s);
 }
 
 }  // extern "C"

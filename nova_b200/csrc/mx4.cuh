@@ -159,37 +159,21 @@ __device__ __forceinline__ void mx4_store(uint8_t* codes_row, uint8_t* scales, i
 }
 
 // ---- rows of fp32 / bf16 in vectors of 8 columns -----------------------------------
-// Columns [8v, 8v + 8) of a row as loaded (zero beyond `cols`).  VEC: the row
-// starts on a 16-byte boundary and cols is a multiple of 8.
+// A vector v holds columns [8v, 8v + 8) of a row, zero behind the last column.
+// The lanes of a warp hold consecutive vectors and load and store together.
+//   VEC: rows start on 16-byte boundaries and cols is a multiple of 8; a lane
+//     moves its vector as 16-byte words.
+//   else: the warp's 256 columns move one column a lane (whole sectors for any
+//     alignment) and change hands through kWarpBuf bytes of the warp's shared
+//     memory.  Eight scalar accesses 8 columns apart per lane instead made
+//     every access of the warp touch 32 sectors (1021 x 5003 fp32 norm: 27 us).
+constexpr int kWarpBuf = 1024;
+__device__ __forceinline__ int lane_of() { return threadIdx.x & 31; }
+
 template <class In>
 struct Raw8 {
     uint4 q[sizeof(In) / 2];
 };
-template <class In, bool VEC>
-__device__ __forceinline__ Raw8<In> load_raw8(const In* row, int v, int cols) {
-    Raw8<In> r;
-    if (VEC) {
-#pragma unroll
-        for (int i = 0; i < static_cast<int>(sizeof(In) / 2); ++i)
-            r.q[i] = 8 * v < cols ? reinterpret_cast<const uint4*>(row + 8 * static_cast<size_t>(v))[i] : make_uint4(0, 0, 0, 0);
-    } else {
-        uint32_t w[2 * sizeof(In)];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const int c = 8 * v + e;
-            if (sizeof(In) == 4) {
-                w[e] = c < cols ? reinterpret_cast<const uint32_t*>(row)[c] : 0u;
-            } else {
-                const uint32_t h = c < cols ? reinterpret_cast<const uint16_t*>(row)[c] : 0u;
-                w[e / 2] = (e & 1) ? (w[e / 2] | (h << 16)) : h;
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < static_cast<int>(sizeof(In) / 2); ++i)
-            r.q[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-    }
-    return r;
-}
 template <class In>
 __device__ __forceinline__ void unpack8(const Raw8<In>& r, float (&v)[8]) {
 #pragma unroll
@@ -210,24 +194,77 @@ __device__ __forceinline__ Raw8<In> pack8(const float (&v)[8]) {
     }
     return r;
 }
+
+// Vectors v0 + i * width, i < NV, of a row; all loads are issued before any use.
+template <class In, bool VEC, int NV>
+__device__ __forceinline__ void load_vecs(Raw8<In> (&r)[NV], const In* row, int v0, int width, int cols, uint8_t* buf) {
+    if (VEC) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int v = v0 + i * width;
+#pragma unroll
+            for (int j = 0; j < static_cast<int>(sizeof(In) / 2); ++j)
+                r[i].q[j] = 8 * v < cols ? reinterpret_cast<const uint4*>(row + 8 * static_cast<size_t>(v))[j] : make_uint4(0, 0, 0, 0);
+        }
+    } else {
+        In* b = reinterpret_cast<In*>(buf);
+        In s[NV][8];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c0 = 8 * (v0 + i * width - lane_of()) + lane_of();
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s[i][e] = c0 + 32 * e < cols ? row[c0 + 32 * e] : In(0);
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            __syncwarp();
+#pragma unroll
+            for (int e = 0; e < 8; ++e) b[32 * e + lane_of()] = s[i][e];
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < static_cast<int>(sizeof(In) / 2); ++j)
+                r[i].q[j] = reinterpret_cast<const uint4*>(b + 8 * lane_of())[j];
+        }
+    }
+}
 template <class In, bool VEC>
-__device__ __forceinline__ void store_raw8(In* row, int v, int cols, const Raw8<In>& r) {
+__device__ __forceinline__ Raw8<In> load_vec(const In* row, int v, int cols, uint8_t* buf) {
+    Raw8<In> r[1];
+    load_vecs<In, VEC, 1>(r, row, v, 0, cols, buf);
+    return r[0];
+}
+template <class In, bool VEC>
+__device__ __forceinline__ void store_vec(In* row, int v, int cols, const Raw8<In>& r, uint8_t* buf) {
     if (VEC) {
         if (8 * v >= cols) return;
 #pragma unroll
         for (int i = 0; i < static_cast<int>(sizeof(In) / 2); ++i)
             reinterpret_cast<uint4*>(row + 8 * static_cast<size_t>(v))[i] = r.q[i];
     } else {
+        In* b = reinterpret_cast<In*>(buf);
+        __syncwarp();
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const int c = 8 * v + e;
-            if (c >= cols) break;
-            const uint4& q = r.q[sizeof(In) == 4 ? e / 4 : 0];
-            const int i = sizeof(In) == 4 ? e % 4 : e / 2;
-            const uint32_t w = i == 0 ? q.x : (i == 1 ? q.y : (i == 2 ? q.z : q.w));
-            if (sizeof(In) == 4) reinterpret_cast<uint32_t*>(row)[c] = w;
-            else reinterpret_cast<uint16_t*>(row)[c] = static_cast<uint16_t>((e & 1) ? w >> 16 : w);
-        }
+        for (int j = 0; j < static_cast<int>(sizeof(In) / 2); ++j) reinterpret_cast<uint4*>(b + 8 * lane_of())[j] = r.q[j];
+        __syncwarp();
+        const int c0 = 8 * (v - lane_of()) + lane_of();
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (c0 + 32 * e < cols) row[c0 + 32 * e] = b[32 * e + lane_of()];
+    }
+}
+// 8 one-byte codes a lane.
+template <bool VEC>
+__device__ __forceinline__ void store_codes8(uint8_t* row, int v, int cols, const uint2& c, uint8_t* buf) {
+    if (VEC) {
+        if (8 * v < cols) *reinterpret_cast<uint2*>(row + 8 * static_cast<size_t>(v)) = c;
+    } else {
+        __syncwarp();
+        reinterpret_cast<uint2*>(buf)[lane_of()] = c;
+        __syncwarp();
+        const int c0 = 8 * (v - lane_of()) + lane_of();
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (c0 + 32 * e < cols) row[c0 + 32 * e] = buf[32 * e + lane_of()];
     }
 }
 

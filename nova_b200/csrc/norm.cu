@@ -39,10 +39,21 @@ struct NormArgs {
     int w_bf16;
 };
 
+// The warp's buffer for rows that are not aligned (one kWarpBuf per warp).
 template <bool VEC>
-__device__ __forceinline__ void load_weight8(const void* w, int w_bf16, int v, int cols, float (&f)[8]) {
-    if (w_bf16) unpack8<uint16_t>(load_raw8<uint16_t, VEC>(static_cast<const uint16_t*>(w), v, cols), f);
-    else unpack8<float>(load_raw8<float, VEC>(static_cast<const float*>(w), v, cols), f);
+__device__ __forceinline__ uint8_t* warp_buf() {
+    if constexpr (VEC) {
+        return nullptr;
+    } else {
+        __shared__ uint4 s_buf[32 * kWarpBuf / 16];
+        return reinterpret_cast<uint8_t*>(s_buf) + (threadIdx.x >> 5) * kWarpBuf;
+    }
+}
+
+template <bool VEC>
+__device__ __forceinline__ void load_weight8(const void* w, int w_bf16, int v, int cols, float (&f)[8], uint8_t* buf) {
+    if (w_bf16) unpack8<uint16_t>(load_vec<uint16_t, VEC>(static_cast<const uint16_t*>(w), v, cols, buf), f);
+    else unpack8<float>(load_vec<float, VEC>(static_cast<const float*>(w), v, cols, buf), f);
 }
 
 // h = x + residual rounded to the type: the stored value is the one normalized.
@@ -62,10 +73,8 @@ __device__ __forceinline__ void block_sum_max(float& s, uint32_t& m, int parity)
     __shared__ float s_sum[2][32];
     __shared__ uint32_t s_max[2][32];
 #pragma unroll
-    for (int o = 16; o; o >>= 1) {
-        s += __shfl_xor_sync(0xffffffffu, s, o);
-        m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-    }
+    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    m = __reduce_max_sync(0xffffffffu, m);
     const int w = threadIdx.x >> 5, l = threadIdx.x & 31;
     if (l == 0) {
         s_sum[parity][w] = s;
@@ -74,12 +83,9 @@ __device__ __forceinline__ void block_sum_max(float& s, uint32_t& m, int parity)
     __syncthreads();
     const int nw = blockDim.x >> 5;
     s = l < nw ? s_sum[parity][l] : 0.0f;
-    m = l < nw ? s_max[parity][l] : 0u;
+    m = __reduce_max_sync(0xffffffffu, l < nw ? s_max[parity][l] : 0u);
 #pragma unroll
-    for (int o = 16; o; o >>= 1) {
-        s += __shfl_xor_sync(0xffffffffu, s, o);
-        m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-    }
+    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
 }
 
 // What a row's reduction gives the encoder.
@@ -110,12 +116,12 @@ __device__ __forceinline__ RowNorm row_norm(float sumsq, uint32_t tmax, int cols
 // Encodes and stores this thread's 8 columns of a row (every lane takes part).
 template <class In, int OUT, bool VEC>
 __device__ __forceinline__ void emit8(const NormArgs& a, int row, int v, int pitch_words, int words, const float (&t)[8],
-                                      const RowNorm& n) {
+                                      const RowNorm& n, uint8_t* buf) {
     if (a.y || OUT == kOutMX) {
         float y[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) y[e] = __fmul_rn(t[e], n.r);
-        if (a.y) store_raw8<In, VEC>(static_cast<In*>(a.y) + static_cast<size_t>(row) * a.cols, v, a.cols, pack8<In>(y));
+        if (a.y) store_vec<In, VEC>(static_cast<In*>(a.y) + static_cast<size_t>(row) * a.cols, v, a.cols, pack8<In>(y), buf);
         if (OUT == kOutMX) {
             uint32_t byte;
             const uint32_t c = mx4_encode<kMXFP4>(y, 0.0f, true, &byte);
@@ -132,29 +138,24 @@ __device__ __forceinline__ void emit8(const NormArgs& a, int row, int v, int pit
         uint32_t c[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) c[i] = ocp_encode2<F>(__fmul_rn(t[2 * i], n.level), __fmul_rn(t[2 * i + 1], n.level));
-        uint8_t* o = a.codes + static_cast<size_t>(row) * a.cols + 8 * static_cast<size_t>(v);
-        if (VEC) {
-            if (8 * v < a.cols) *reinterpret_cast<uint2*>(o) = make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (8 * v + e < a.cols) o[e] = static_cast<uint8_t>(c[e / 2] >> (8 * (e & 1)));
-        }
+        store_codes8<VEC>(a.codes + static_cast<size_t>(row) * a.cols, v, a.cols, make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16)), buf);
     }
 }
 
 // One block per row in two passes: the reduction, then the encoding of the row
-// read again (from sum where it is stored).  Any width and alignment.
+// read again (from sum where it is stored).  For rows too wide for k_norm_rows.
 template <class In, int OUT, bool VEC>
 __global__ void __launch_bounds__(256) k_norm_two_pass(const NormArgs a) {
     pdl_launch_dependents();
     pdl_wait();
+    uint8_t* buf = warp_buf<VEC>();
     constexpr int F = OUT == kOutNV ? kNVFP4 : kMXFP4;
     const int nvec = (a.cols + 7) / 8;
     const bool four = OUT == kOutMX || OUT == kOutNV;
     const int words = four ? mx4_words(a.cols, Mx4Traits<F>::block) : 0;
     const int pitch_words = static_cast<int>(mx4_pitch(a.cols) / 4);
     const int nstep = four ? words * Mx4Traits<F>::word_lanes : nvec;
+    const int lane = lane_of();
     int parity = 0;
     for (long long rl = blockIdx.x; rl < a.rows; rl += gridDim.x, parity ^= 1) {
         const int row = static_cast<int>(rl);
@@ -162,17 +163,17 @@ __global__ void __launch_bounds__(256) k_norm_two_pass(const NormArgs a) {
         const In* res = a.res ? static_cast<const In*>(a.res) + row * a.res_stride : nullptr;
         In* sum = a.sum ? static_cast<In*>(a.sum) + static_cast<size_t>(row) * a.cols : nullptr;
         auto load_h = [&](int v) {
-            const Raw8<In> h = load_raw8<In, VEC>(x, v, a.cols);
-            return res ? add8<In>(h, load_raw8<In, VEC>(res, v, a.cols)) : h;
+            const Raw8<In> h = load_vec<In, VEC>(x, v, a.cols, buf);
+            return res ? add8<In>(h, load_vec<In, VEC>(res, v, a.cols, buf)) : h;
         };
         float ss = 0.0f;
         uint32_t tm = 0;
-        for (int v = threadIdx.x; v < nvec; v += blockDim.x) {
+        for (int v = threadIdx.x; v - lane < nvec; v += blockDim.x) {
             const Raw8<In> hr = load_h(v);
-            if (sum) store_raw8<In, VEC>(sum, v, a.cols, hr);
+            if (sum) store_vec<In, VEC>(sum, v, a.cols, hr, buf);
             float h[8], w[8];
             unpack8<In>(hr, h);
-            load_weight8<VEC>(a.w, a.w_bf16, v, a.cols, w);
+            load_weight8<VEC>(a.w, a.w_bf16, v, a.cols, w, buf);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 ss = __fmaf_rn(h[e], h[e], ss);
@@ -180,17 +181,88 @@ __global__ void __launch_bounds__(256) k_norm_two_pass(const NormArgs a) {
             }
             tm = max(tm, amax_bits8(w));
         }
-        block_sum_max(ss, tm, parity);
+        block_sum_max(ss, tm, parity);  // (its barrier also orders the unaligned rows' stores before the loads below)
         float scale = 0.0f;
         const RowNorm n = row_norm<OUT>(ss, tm, a.cols, a.eps, &scale);
         if (threadIdx.x == 0 && (OUT <= kOutINT8 || OUT == kOutNV)) a.scales[row] = scale;
-        for (int v = threadIdx.x; v - static_cast<int>(threadIdx.x & 31) < nstep; v += blockDim.x) {
+        for (int v = threadIdx.x; v - lane < nstep; v += blockDim.x) {
             float t[8], w[8];
-            unpack8<In>(sum ? load_raw8<In, VEC>(sum, v, a.cols) : load_h(v), t);
-            load_weight8<VEC>(a.w, a.w_bf16, v, a.cols, w);
+            unpack8<In>(sum ? load_vec<In, VEC>(sum, v, a.cols, buf) : load_h(v), t);
+            load_weight8<VEC>(a.w, a.w_bf16, v, a.cols, w, buf);
 #pragma unroll
             for (int e = 0; e < 8; ++e) t[e] = __fmul_rn(t[e], w[e]);
-            emit8<In, OUT, VEC>(a, row, v, pitch_words, words, t, n);
+            emit8<In, OUT, VEC>(a, row, v, pitch_words, words, t, n, buf);
+        }
+    }
+}
+
+// Rows held in registers: a row is read once, 8 columns a vector and NV vectors
+// a thread, by one warp (WARP, 8 rows a block) or one block; the block's
+// threads are as many as the row needs.
+template <class In, int OUT, bool VEC, int NV, bool WARP>
+__global__ void __launch_bounds__(WARP ? 256 : 1024) k_norm_rows(const NormArgs a) {
+    pdl_launch_dependents();
+    uint8_t* buf = warp_buf<VEC>();
+    constexpr int F = OUT == kOutNV ? kNVFP4 : kMXFP4;
+    const bool four = OUT == kOutMX || OUT == kOutNV;
+    const int words = four ? mx4_words(a.cols, Mx4Traits<F>::block) : 0;
+    const int pitch_words = static_cast<int>(mx4_pitch(a.cols) / 4);
+    const int width = WARP ? 32 : blockDim.x;
+    const int t0 = WARP ? threadIdx.x & 31 : threadIdx.x;
+    const int per = WARP ? blockDim.x >> 5 : 1;  // rows a block takes at once
+    pdl_wait();
+    int parity = 0;
+    for (long long rl = static_cast<long long>(blockIdx.x) * per + (WARP ? threadIdx.x >> 5 : 0); rl < a.rows;
+         rl += static_cast<long long>(gridDim.x) * per, parity ^= 1) {
+        const int row = static_cast<int>(rl);
+        const In* x = static_cast<const In*>(a.x) + row * a.x_stride;
+        Raw8<In> h[NV];
+        load_vecs<In, VEC, NV>(h, x, t0, width, a.cols, buf);
+        if (a.res) {
+            const In* res = static_cast<const In*>(a.res) + row * a.res_stride;
+            Raw8<In> q[NV];
+            load_vecs<In, VEC, NV>(q, res, t0, width, a.cols, buf);
+#pragma unroll
+            for (int i = 0; i < NV; ++i) h[i] = add8<In>(h[i], q[i]);
+            if (a.sum) {
+                In* sum = static_cast<In*>(a.sum) + static_cast<size_t>(row) * a.cols;
+#pragma unroll
+                for (int i = 0; i < NV; ++i) store_vec<In, VEC>(sum, t0 + i * width, a.cols, h[i], buf);
+            }
+        }
+        float ss = 0.0f;
+        uint32_t tm = 0;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            float f[8], w[8];
+            unpack8<In>(h[i], f);
+            load_weight8<VEC>(a.w, a.w_bf16, t0 + i * width, a.cols, w, buf);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                ss = __fmaf_rn(f[e], f[e], ss);
+                w[e] = __fmul_rn(f[e], w[e]);
+            }
+            tm = max(tm, amax_bits8(w));
+        }
+        if (WARP) {
+#pragma unroll
+            for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+            tm = __reduce_max_sync(0xffffffffu, tm);
+        } else {
+            block_sum_max(ss, tm, parity);
+        }
+        float scale = 0.0f;
+        const RowNorm n = row_norm<OUT>(ss, tm, a.cols, a.eps, &scale);
+        if (t0 == 0 && (OUT <= kOutINT8 || OUT == kOutNV)) a.scales[row] = scale;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int v = t0 + i * width;
+            float f[8], w[8];
+            unpack8<In>(h[i], f);
+            load_weight8<VEC>(a.w, a.w_bf16, v, a.cols, w, buf);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] = __fmul_rn(f[e], w[e]);
+            emit8<In, OUT, VEC>(a, row, v, pitch_words, words, f, n, buf);
         }
     }
 }
@@ -232,13 +304,28 @@ __device__ __forceinline__ void block_sum2(float& s, float& g, int parity) {
     }
 }
 
-// dx = dsum + r g - h (r^3 mean(g h)), g = dy w, one block per row in two
-// passes; r of every row also goes to `rs` for the weight's gradient.
+// Row terms of the gradient: dx = dsum + r (g - h c), c = r mean(g n), n = h r
+// (the bounded form: |mean(g n)| <= max |g|).
+struct RowGrad {
+    float r, c;
+};
+__device__ __forceinline__ RowGrad row_grad(float sumsq, float sgh, int cols, float eps) {
+    const float n = static_cast<float>(cols);
+    RowGrad q;
+    q.r = __frsqrt_rn(__fadd_rn(__fdiv_rn(sumsq, n), eps));
+    q.c = __fmul_rn(__fdiv_rn(__fmul_rn(sgh, q.r), n), q.r);
+    return q;
+}
+
+// One block per row in two passes, for rows too wide for k_norm_grad; r of every
+// row also goes to `rs` for the weight's gradient.
 template <class In, bool VEC>
 __global__ void __launch_bounds__(256) k_norm_grad_rows(const GradArgs a, float* __restrict__ rs) {
     pdl_launch_dependents();
     pdl_wait();
+    uint8_t* buf = warp_buf<VEC>();
     const int nvec = (a.cols + 7) / 8;
+    const int lane = lane_of();
     int parity = 0;
     for (long long rl = blockIdx.x; rl < a.rows; rl += gridDim.x, parity ^= 1) {
         const int row = static_cast<int>(rl);
@@ -246,11 +333,11 @@ __global__ void __launch_bounds__(256) k_norm_grad_rows(const GradArgs a, float*
         const size_t at = static_cast<size_t>(row) * a.cols;
         const In* dyp = static_cast<const In*>(a.dy) + at;
         float ss = 0.0f, sg = 0.0f;
-        for (int v = threadIdx.x; v < nvec; v += blockDim.x) {
+        for (int v = threadIdx.x; v - lane < nvec; v += blockDim.x) {
             float h[8], g[8], w[8];
-            unpack8<In>(load_raw8<In, VEC>(hp, v, a.cols), h);
-            unpack8<In>(load_raw8<In, VEC>(dyp, v, a.cols), g);
-            load_weight8<VEC>(a.w, a.w_bf16, v, a.cols, w);
+            unpack8<In>(load_vec<In, VEC>(hp, v, a.cols, buf), h);
+            unpack8<In>(load_vec<In, VEC>(dyp, v, a.cols, buf), g);
+            load_weight8<VEC>(a.w, a.w_bf16, v, a.cols, w, buf);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 ss = __fmaf_rn(h[e], h[e], ss);
@@ -258,26 +345,122 @@ __global__ void __launch_bounds__(256) k_norm_grad_rows(const GradArgs a, float*
             }
         }
         block_sum2(ss, sg, parity);
-        const float n = static_cast<float>(a.cols);
-        const float r = __frsqrt_rn(__fadd_rn(__fdiv_rn(ss, n), a.eps));
-        if (threadIdx.x == 0) rs[row] = r;
+        const RowGrad q = row_grad(ss, sg, a.cols, a.eps);
+        if (threadIdx.x == 0) rs[row] = q.r;
         if (!a.dx) continue;
-        // c h = r (mean(g n) n) with n = h r, the bounded form: |mean(g n)| <= max |g| sqrt(cols)
-        const float c = __fmul_rn(__fdiv_rn(__fmul_rn(sg, r), n), r);
-        for (int v = threadIdx.x; v < nvec; v += blockDim.x) {
-            float h[8], g[8], w[8];
-            unpack8<In>(load_raw8<In, VEC>(hp, v, a.cols), h);
-            unpack8<In>(load_raw8<In, VEC>(dyp, v, a.cols), g);
-            load_weight8<VEC>(a.w, a.w_bf16, v, a.cols, w);
+        for (int v = threadIdx.x; v - lane < nvec; v += blockDim.x) {
+            float h[8], g[8], w[8], d[8];
+            unpack8<In>(load_vec<In, VEC>(hp, v, a.cols, buf), h);
+            unpack8<In>(load_vec<In, VEC>(dyp, v, a.cols, buf), g);
+            load_weight8<VEC>(a.w, a.w_bf16, v, a.cols, w, buf);
+            if (a.dsum) unpack8<In>(load_vec<In, VEC>(static_cast<const In*>(a.dsum) + at, v, a.cols, buf), d);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) g[e] = __fmul_rn(r, __fmaf_rn(-h[e], c, __fmul_rn(g[e], w[e])));
-            if (a.dsum) {
-                float d[8];
-                unpack8<In>(load_raw8<In, VEC>(static_cast<const In*>(a.dsum) + at, v, a.cols), d);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) g[e] = __fadd_rn(g[e], d[e]);
+            for (int e = 0; e < 8; ++e) {
+                g[e] = __fmul_rn(q.r, __fmaf_rn(-h[e], q.c, __fmul_rn(g[e], w[e])));
+                if (a.dsum) g[e] = __fadd_rn(g[e], d[e]);
             }
-            store_raw8<In, VEC>(static_cast<In*>(a.dx) + at, v, a.cols, pack8<In>(g));
+            store_vec<In, VEC>(static_cast<In*>(a.dx) + at, v, a.cols, pack8<In>(g), buf);
+        }
+    }
+}
+
+// Rows held in registers, read once: dx, and the weight's gradient summed over
+// the block's rows (blockIdx.x, + gridDim.x, ...) in registers, one partial row a
+// block.  WARP: a warp per row; the block's warps are added in order at the end.
+template <class In, bool VEC, int NV, bool WARP>
+__global__ void __launch_bounds__(WARP ? 256 : 512) k_norm_grad(const GradArgs a, float* __restrict__ part) {
+    pdl_launch_dependents();
+    uint8_t* buf = warp_buf<VEC>();
+    const int width = WARP ? 32 : blockDim.x;
+    const int t0 = WARP ? lane_of() : threadIdx.x;
+    const int per = WARP ? blockDim.x >> 5 : 1;
+    pdl_wait();
+    float acc[NV][8];
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc[i][e] = 0.0f;
+    int parity = 0;
+    for (long long rl = static_cast<long long>(blockIdx.x) * per + (WARP ? threadIdx.x >> 5 : 0); rl < a.rows;
+         rl += static_cast<long long>(gridDim.x) * per, parity ^= 1) {
+        const size_t at = static_cast<size_t>(rl) * a.cols;
+        Raw8<In> hr[NV], gr[NV], dr[NV];
+        load_vecs<In, VEC, NV>(hr, static_cast<const In*>(a.h) + static_cast<size_t>(rl) * a.h_stride, t0, width, a.cols, buf);
+        load_vecs<In, VEC, NV>(gr, static_cast<const In*>(a.dy) + at, t0, width, a.cols, buf);
+        if (a.dsum && a.dx) load_vecs<In, VEC, NV>(dr, static_cast<const In*>(a.dsum) + at, t0, width, a.cols, buf);
+        float ss = 0.0f, sg = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            float h[8], g[8], w[8];
+            unpack8<In>(hr[i], h);
+            unpack8<In>(gr[i], g);
+            load_weight8<VEC>(a.w, a.w_bf16, t0 + i * width, a.cols, w, buf);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                ss = __fmaf_rn(h[e], h[e], ss);
+                sg = __fmaf_rn(__fmul_rn(g[e], w[e]), h[e], sg);
+            }
+        }
+        if (WARP) {
+#pragma unroll
+            for (int o = 16; o; o >>= 1) {
+                ss += __shfl_xor_sync(0xffffffffu, ss, o);
+                sg += __shfl_xor_sync(0xffffffffu, sg, o);
+            }
+        } else {
+            block_sum2(ss, sg, parity);
+        }
+        const RowGrad q = row_grad(ss, sg, a.cols, a.eps);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int v = t0 + i * width;
+            float h[8], g[8];
+            unpack8<In>(hr[i], h);
+            unpack8<In>(gr[i], g);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) acc[i][e] = __fmaf_rn(__fmul_rn(h[e], q.r), g[e], acc[i][e]);
+            if (a.dx) {
+                float w[8], d[8];
+                load_weight8<VEC>(a.w, a.w_bf16, v, a.cols, w, buf);
+                if (a.dsum) unpack8<In>(dr[i], d);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    g[e] = __fmul_rn(q.r, __fmaf_rn(-h[e], q.c, __fmul_rn(g[e], w[e])));
+                    if (a.dsum) g[e] = __fadd_rn(g[e], d[e]);
+                }
+                store_vec<In, VEC>(static_cast<In*>(a.dx) + at, v, a.cols, pack8<In>(g), buf);
+            }
+        }
+    }
+    if (!part) return;
+    float* mine = part + static_cast<size_t>(blockIdx.x) * a.cols;
+    if constexpr (WARP) {
+        __shared__ float s_acc[NV * 256];
+        for (int k = 0; k < per; ++k) {
+            if (static_cast<int>(threadIdx.x >> 5) == k) {
+#pragma unroll
+                for (int i = 0; i < NV; ++i)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        float* s = s_acc + i * 256 + e * 32 + t0;  // column (t0 + 32 i) * 8 + e
+                        *s = k == 0 ? acc[i][e] : __fadd_rn(*s, acc[i][e]);
+                    }
+            }
+            __syncthreads();
+        }
+        for (int c = threadIdx.x; c < a.cols; c += blockDim.x) mine[c] = s_acc[c / 256 * 256 + (c & 7) * 32 + (c / 8 & 31)];
+    } else {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = 8 * (t0 + i * width);
+            if (VEC) {
+                if (c < a.cols) {
+                    reinterpret_cast<float4*>(mine + c)[0] = make_float4(acc[i][0], acc[i][1], acc[i][2], acc[i][3]);
+                    reinterpret_cast<float4*>(mine + c)[1] = make_float4(acc[i][4], acc[i][5], acc[i][6], acc[i][7]);
+                }
+            } else {
+                store_vec<float, VEC>(mine, t0 + i * width, a.cols, pack8<float>(acc[i]), buf);
+            }
         }
     }
 }
@@ -306,14 +489,26 @@ __global__ void __launch_bounds__(256) k_norm_grad_weight(const GradArgs a, cons
     }
     part[static_cast<size_t>(blockIdx.y) * a.cols + c] = s;
 }
-__global__ void __launch_bounds__(256) k_sum_chunks(const float* __restrict__ part, int chunks, int cols, float* __restrict__ dw) {
+// dw[c] = sum of the partial rows: 32 columns a block, warp k adds rows k, k + 32,
+// ... and the warps are added in order.
+__global__ void __launch_bounds__(1024) k_sum_chunks(const float* __restrict__ part, int chunks, int cols, float* __restrict__ dw) {
+    __shared__ float s_part[32][33];
     pdl_launch_dependents();
     pdl_wait();
-    const int c = blockIdx.x * 256 + threadIdx.x;
-    if (c >= cols) return;
+    const int c = blockIdx.x * 32 + lane_of(), k0 = threadIdx.x >> 5;
     float s = 0.0f;
-    for (int k = 0; k < chunks; ++k) s = __fadd_rn(s, part[static_cast<size_t>(k) * cols + c]);
-    dw[c] = s;
+    if (c < cols) {
+#pragma unroll 4
+        for (int k = k0; k < chunks; k += 32) s = __fadd_rn(s, part[static_cast<size_t>(k) * cols + c]);
+    }
+    s_part[k0][lane_of()] = s;
+    __syncthreads();
+    if (k0 == 0 && c < cols) {
+        s = s_part[0][lane_of()];
+#pragma unroll
+        for (int k = 1; k < 32; ++k) s = __fadd_rn(s, s_part[k][lane_of()]);
+        dw[c] = s;
+    }
 }
 
 // ---- host side -------------------------------------------------------------------
@@ -338,8 +533,33 @@ nq_status_t check_desc(const char* who, const nq_rmsnorm_desc_t* d, size_t* xs, 
     return NQ_SUCCESS;
 }
 
+template <class In, int OUT, bool VEC, int NV, bool WARP>
+nq_status_t launch_norm_rows(const NormArgs& a, int threads, const DeviceInfo& di, cudaStream_t s, const char* who) {
+    auto kern = k_norm_rows<In, OUT, VEC, NV, WARP>;
+    int per_sm = 0;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, threads, 0) != cudaSuccess || per_sm < 1) {
+        cudaGetLastError();
+        per_sm = 1;
+    }
+    const long long blocks = WARP ? (static_cast<long long>(a.rows) + threads / 32 - 1) / (threads / 32) : a.rows;
+    const int grid = static_cast<int>(std::min<long long>(blocks, static_cast<long long>(di.sm_count) * per_sm));
+    return cuda_status(launch_pdl(kern, dim3(grid), dim3(threads), 0, s, a), who);
+}
+
 template <class In, int OUT, bool VEC>
 nq_status_t launch_norm(const NormArgs& a, const DeviceInfo& di, cudaStream_t s, const char* who) {
+    constexpr int NVMAX = sizeof(In) == 2 ? 4 : 2;  // 64 bytes a thread of each tensor
+    int nvec = (a.cols + 7) / 8;
+    if (OUT == kOutMX) nvec = mx4_words(a.cols, 32) * 16;  // whole scale words
+    if (OUT == kOutNV) nvec = mx4_words(a.cols, 16) * 8;
+    if (nvec <= 32 * NVMAX) {
+        if (nvec <= 32) return launch_norm_rows<In, OUT, VEC, 1, true>(a, 256, di, s, who);
+        return launch_norm_rows<In, OUT, VEC, NVMAX, true>(a, 256, di, s, who);
+    }
+    if (a.rows < 2 * di.sm_count && nvec <= 1024)
+        return launch_norm_rows<In, OUT, VEC, 1, false>(a, (nvec + 31) / 32 * 32, di, s, who);
+    const int threads = ((nvec + NVMAX - 1) / NVMAX + 31) / 32 * 32;
+    if (threads <= 1024) return launch_norm_rows<In, OUT, VEC, NVMAX, false>(a, threads, di, s, who);
     const int grid = static_cast<int>(std::min<long long>(a.rows, static_cast<long long>(di.sm_count) * 8));
     return cuda_status(launch_pdl(k_norm_two_pass<In, OUT, VEC>, dim3(grid), dim3(256), 0, s, a), who);
 }
@@ -395,9 +615,40 @@ nq_status_t norm_impl(const char* who, const nq_rmsnorm_desc_t* d, const void* x
     }
 }
 
-template <class In>
-nq_status_t grad_impl(const GradArgs& a, float* dw, bool vec, const DeviceInfo& di, cudaStream_t s) {
-    const char* who = "nq_rmsnorm_backward";
+nq_status_t sum_chunks(const float* part, int chunks, int cols, float* dw, cudaStream_t s) {
+    return cuda_status(launch_pdl(k_sum_chunks, dim3((cols + 31) / 32), dim3(1024), 0, s, part, chunks, cols, dw),
+                       "nq_rmsnorm_backward (weight)");
+}
+
+template <class In, bool VEC, int NV, bool WARP>
+nq_status_t launch_grad(const GradArgs& a, float* dw, int threads, const DeviceInfo& di, cudaStream_t s) {
+    auto kern = k_norm_grad<In, VEC, NV, WARP>;
+    int per_sm = 0;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, threads, 0) != cudaSuccess || per_sm < 1) {
+        cudaGetLastError();
+        per_sm = 1;
+    }
+    const long long blocks = WARP ? (static_cast<long long>(a.rows) + threads / 32 - 1) / (threads / 32) : a.rows;
+    const int grid = static_cast<int>(std::min<long long>(blocks, static_cast<long long>(di.sm_count) * per_sm));
+    void* part = nullptr;
+    nq_status_t st = NQ_SUCCESS;
+    if (dw) st = scratch_alloc(&part, static_cast<size_t>(grid) * a.cols * 4, s);
+    if (st != NQ_SUCCESS) return st;
+    st = cuda_status(launch_pdl(kern, dim3(grid), dim3(threads), 0, s, a, static_cast<float*>(part)), "nq_rmsnorm_backward");
+    if (st == NQ_SUCCESS && dw) st = sum_chunks(static_cast<const float*>(part), grid, a.cols, dw, s);
+    scratch_free(part, s);
+    return st;
+}
+
+template <class In, bool VEC>
+nq_status_t grad_impl(const GradArgs& a, float* dw, const DeviceInfo& di, cudaStream_t s) {
+    constexpr int NVMAX = sizeof(In) == 2 ? 4 : 2;  // 64 bytes a thread of each tensor
+    const int nvec = (a.cols + 7) / 8;
+    if (nvec <= 32) return launch_grad<In, VEC, 1, true>(a, dw, 256, di, s);
+    if (nvec <= 32 * NVMAX) return launch_grad<In, VEC, NVMAX, true>(a, dw, 256, di, s);
+    if (nvec <= 512) return launch_grad<In, VEC, 1, false>(a, dw, (nvec + 31) / 32 * 32, di, s);
+    const int threads = ((nvec + NVMAX - 1) / NVMAX + 31) / 32 * 32;
+    if (threads <= 512) return launch_grad<In, VEC, NVMAX, false>(a, dw, threads, di, s);
     const int chunks = static_cast<int>(std::min<long long>(64, a.rows));
     const int per = (a.rows + chunks - 1) / chunks;
     void* scratch = nullptr;
@@ -407,16 +658,14 @@ nq_status_t grad_impl(const GradArgs& a, float* dw, bool vec, const DeviceInfo& 
     float* rs = static_cast<float*>(scratch);
     float* part = reinterpret_cast<float*>(static_cast<char*>(scratch) + rs_bytes);
     const int grid = static_cast<int>(std::min<long long>(a.rows, static_cast<long long>(di.sm_count) * 8));
-    cudaError_t e = vec ? launch_pdl(k_norm_grad_rows<In, true>, dim3(grid), dim3(256), 0, s, a, rs)
-                        : launch_pdl(k_norm_grad_rows<In, false>, dim3(grid), dim3(256), 0, s, a, rs);
-    if (e == cudaSuccess && dw) {
-        const int cb = (a.cols + 255) / 256;
-        e = launch_pdl(k_norm_grad_weight<In>, dim3(cb, chunks), dim3(256), 0, s, a, static_cast<const float*>(rs), per, part);
-        if (e == cudaSuccess)
-            e = launch_pdl(k_sum_chunks, dim3(cb), dim3(256), 0, s, static_cast<const float*>(part), chunks, a.cols, dw);
-    }
+    cudaError_t e = launch_pdl(k_norm_grad_rows<In, VEC>, dim3(grid), dim3(256), 0, s, a, rs);
+    if (e == cudaSuccess && dw)
+        e = launch_pdl(k_norm_grad_weight<In>, dim3((a.cols + 255) / 256, chunks), dim3(256), 0, s, a,
+                       static_cast<const float*>(rs), per, part);
+    st = cuda_status(e, "nq_rmsnorm_backward");
+    if (st == NQ_SUCCESS && dw) st = sum_chunks(part, chunks, a.cols, dw, s);
     scratch_free(scratch, s);
-    return cuda_status(e, who);
+    return st;
 }
 
 }  // namespace
@@ -466,7 +715,8 @@ nq_status_t nq_rmsnorm_backward(const nq_rmsnorm_desc_t* desc, const void* h, co
                      nq::aligned16(grad_y) && nq::aligned16(grad_sum) && nq::aligned16(grad_x);
     const nq::GradArgs a{h, weight, grad_y, grad_sum, grad_x, desc->rows, desc->cols, xs, desc->eps,
                          desc->weight_dtype == NQ_BF16};
-    return bf ? nq::grad_impl<uint16_t>(a, grad_weight, vec, di, s) : nq::grad_impl<float>(a, grad_weight, vec, di, s);
+    if (bf) return vec ? nq::grad_impl<uint16_t, true>(a, grad_weight, di, s) : nq::grad_impl<uint16_t, false>(a, grad_weight, di, s);
+    return vec ? nq::grad_impl<float, true>(a, grad_weight, di, s) : nq::grad_impl<float, false>(a, grad_weight, di, s);
 }
 
 }  // extern "C"
