@@ -405,8 +405,8 @@ nq_status_t nq_dequantize_rows_mx4(const uint8_t* codes, const uint8_t* block_sc
 /* out[m, n] = epi( sum_k A[m, k] * B[n, k] ): A m x k and B n x k both in the
  * 4-bit storage above (B "packed", NQ_B_NK), block scales applied inside the
  * product (tcgen05 kind::mxf4 / kind::mxf4nvf4 with block scaling), fp32 sums.
- *   epi(acc) = ((acc * alpha) [* row_scale[m]]) [* col_scale[n]] [+ bias[n]]
- * as in nq_gemm; the NVFP4 row scales of A and B are passed as row_scale and
+ *   epi(acc) = (acc * (alpha [* row_scale[m]])) [* col_scale[n]] [+ bias[n]]
+ * with one fp32 rounding a step; the NVFP4 row scales of A and B are passed as row_scale and
  * col_scale.  out: m x n dense, NQ_F32 or NQ_BF16, any m, n, k >= 0 (k = 0: the
  * sum is 0). */
 typedef struct {

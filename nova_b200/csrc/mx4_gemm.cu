@@ -39,9 +39,20 @@ struct MxEpi {
     const float* bias;
 };
 
-// ((acc * alpha) * row) * col + bias, one rounding per step (absent vectors are 1 and -0).
-__device__ __forceinline__ float mx_epi(float acc, float alpha, float rs, float cs, float b) {
-    return __fadd_rn(__fmul_rn(__fmul_rn(__fmul_rn(acc, alpha), rs), cs), b);
+// (acc * (alpha * row)) * col + bias, one rounding per step (absent vectors are 1 and -0).
+__device__ __forceinline__ float mx_epi(float acc, float row, float cs, float b) {
+    return __fadd_rn(__fmul_rn(__fmul_rn(acc, row), cs), b);
+}
+// Two fp32 operations an instruction.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    uint64_t r, x = *reinterpret_cast<uint64_t*>(&a), y = *reinterpret_cast<uint64_t*>(&b);
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+    return *reinterpret_cast<float2*>(&r);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    uint64_t r, x = *reinterpret_cast<uint64_t*>(&a), y = *reinterpret_cast<uint64_t*>(&b);
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+    return *reinterpret_cast<float2*>(&r);
 }
 
 // Keeps the compiler from using registers that tcgen05.ld fills before the wait
@@ -78,15 +89,17 @@ struct PairCfg {
     static constexpr int COLS = EPI_WARPS * 256;      // per warp: a chunk's column scales and biases
     static constexpr int SMEM = 1024 + STAGES * STAGE + EPI_WARPS * 2 * SLOT + COLS + 256;
     static constexpr int THREADS = 32 * (2 + EPI_WARPS);
-    // Tensor memory: the accumulators of consecutive tiles share 96 of their
-    // columns, [0, 256) and [160, 416); behind them two slots of a stage's scales.
-    static constexpr int ACC1 = 160;
-    static constexpr int SF = 416;
-    static constexpr int SF_SLOT = 48;
+    // Tensor memory: the accumulators of consecutive tiles share half of their
+    // columns, [0, 256) and [128, 384); behind them a ring of 10 scale words (4
+    // columns for A, 8 for B): two and a half stages of NVFP4, all five of MXFP4.
+    static constexpr int ACC1 = 128;
+    static constexpr int SF = 384;
+    static constexpr int RING = 10;
+    static constexpr bool SF_WAIT = WORDS * STAGES > RING;
 };
 
-constexpr int M_BAND = 16;
-// Bands of 16 row tiles; inside a band the row tiles run fastest, so that the
+constexpr int M_BAND = 32;
+// Bands of 32 row tiles; inside a band the row tiles run fastest, so that the
 // clusters in flight share few panels of A and B.
 __device__ __forceinline__ void pair_tile(int tile, int m_tiles, int n_tiles, int& mb, int& nb) {
     const int band = tile / (M_BAND * n_tiles);
@@ -97,17 +110,32 @@ __device__ __forceinline__ void pair_tile(int tile, int m_tiles, int n_tiles, in
 }
 
 // The i-th 32-column chunk of a tile that an epilogue warp of column group g
-// drains: the columns that the next tile's accumulator overlays come first.
+// drains: the half that the next tile's accumulator overlays comes first.
 __device__ __forceinline__ int chunk_of(int acc, int g, int i) {
-    if (acc == 0) return g == 0 ? (i == 0 ? 5 : i - 1) : (i < 2 ? 6 + i : 1 + i);  // shared: chunks 5..7
-    return g == 0 ? (i == 0 ? 0 : 2 + i) : (i < 2 ? 1 + i : 4 + i);                // shared: chunks 0..2
+    return (((i < 2) == (acc == 0)) ? 4 : 0) + 2 * g + (i & 1);
+}
+
+// Tiles [0, whole) are dealt round-robin; where the rest fill at most half the
+// clusters, each of them is done as two 256 x 128 halves by two clusters.
+struct PairUnit {
+    int tile;
+    int half;  // 0: the whole tile, 1 / 2: its columns [0, 128) / [128, 256)
+};
+__device__ __forceinline__ int pair_units(int tiles, int whole, int cluster, int nclusters) {
+    const int n = whole > cluster ? (whole - cluster + nclusters - 1) / nclusters : 0;
+    return n + (cluster < 2 * (tiles - whole) ? 1 : 0);
+}
+__device__ __forceinline__ PairUnit pair_unit(int whole, int cluster, int nclusters, int j) {
+    const int tile = cluster + j * nclusters;
+    return tile < whole ? PairUnit{tile, 0} : PairUnit{whole + cluster / 2, 1 + (cluster & 1)};
 }
 
 template <bool MX, bool BF16>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<MX, BF16>::THREADS, 1)
     k_mx4_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-               const __grid_constant__ CUtensorMap tmSA, const __grid_constant__ CUtensorMap tmSB,
-               const __grid_constant__ CUtensorMap tmC, int M, int N, int K, MxEpi ep, uint32_t* err) {
+               const __grid_constant__ CUtensorMap tmBh, const __grid_constant__ CUtensorMap tmSA,
+               const __grid_constant__ CUtensorMap tmSB, const __grid_constant__ CUtensorMap tmC, int M, int N, int K,
+               int whole, MxEpi ep, uint32_t* err) {
     using C = PairCfg<MX, BF16>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -123,7 +151,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<MX, BF16>::T
     uint64_t* tfull = empty + C::STAGES;    // [2] MMA -> each CTA's epilogue
     uint64_t* tempty = tfull + 2;           // leader: 16 epilogue warps -> MMA, once a tile
     uint64_t* done = tempty + 1;            // leader: MMA drain
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+    uint64_t* mid = done + 1;               // [STAGES] leader: a stage's first two MMAs are complete
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mid + C::STAGES);
 
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
@@ -132,8 +161,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<MX, BF16>::T
     const int nclusters = gridDim.x >> 1;
     const int m_tiles = (M + 255) / 256;
     const int n_tiles = (N + 255) / 256;
-    const int num_tiles = m_tiles * n_tiles;
     const int kblocks = (K + BK - 1) / BK;
+    const int units = pair_units(m_tiles * n_tiles, whole, cluster, nclusters);
 
     // Up to pdl_wait() nothing touches memory that an earlier kernel may write.
     pdl_launch_dependents();
@@ -141,6 +170,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<MX, BF16>::T
         for (int s = 0; s < C::STAGES; ++s) {
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], 1);
+            mbar_init(&mid[s], 1);
         }
         mbar_init(&tfull[0], 1);
         mbar_init(&tfull[1], 1);
@@ -151,6 +181,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<MX, BF16>::T
     if (warp == 0 && lane == 0) {
         tma_prefetch_desc(&tmA);
         tma_prefetch_desc(&tmB);
+        tma_prefetch_desc(&tmBh);
         tma_prefetch_desc(&tmSA);
         tma_prefetch_desc(&tmSB);
         if (ep.tma_out) tma_prefetch_desc(&tmC);
@@ -172,18 +203,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<MX, BF16>::T
             int stage = 0;
             uint32_t phase = 0;
             bool ok = true;
-            for (int tile = cluster; tile < num_tiles && ok; tile += nclusters) {
+            for (int j = 0; j < units && ok; ++j) {
+                const PairUnit un = pair_unit(whole, cluster, nclusters, j);
                 int mb, nb;
-                pair_tile(tile, m_tiles, n_tiles, mb, nb);
+                pair_tile(un.tile, m_tiles, n_tiles, mb, nb);
+                const int hi = un.half == 2 ? 1 : 0;
+                const int brow = nb * 256 + (un.half ? 128 * hi + static_cast<int>(rank) * 64 : static_cast<int>(rank) * 128);
                 for (int kb = 0; kb < kblocks; ++kb) {
                     if (!mbar_wait(&empty[stage], phase ^ 1u, err)) { ok = false; break; }
-                    if (rank == 0) mbar_arrive_expect_tx(&full[stage], 2 * C::STAGE);
+                    if (rank == 0) mbar_arrive_expect_tx(&full[stage], 2 * (un.half ? C::STAGE - C::B_BYTES / 2 : C::STAGE));
                     const uint32_t fb = full_leader + 8u * stage;
                     tma_load_2d_pair(sA + stage * C::A_BYTES, &tmA, fb, kb * BKB, mb * 256 + rank * 128);
-                    tma_load_2d_pair(sB + stage * C::B_BYTES, &tmB, fb, kb * BKB, nb * 256 + rank * 128);
+                    tma_load_2d_pair(sB + stage * C::B_BYTES, un.half ? &tmBh : &tmB, fb, kb * BKB, brow);
                     // 8-byte elements: 64 to a 512-byte scale tile; row blocks of 128
                     tma_load_2d_pair(sSA + stage * C::SFA_BYTES, &tmSA, fb, kb * C::WORDS * 64, mb * 2 + rank);
-                    tma_load_2d_pair(sSB + stage * C::SFB_BYTES, &tmSB, fb, kb * C::WORDS * 64, nb * 2);
+                    tma_load_2d_pair(sSB + stage * C::SFB_BYTES, &tmSB, fb, kb * C::WORDS * 64, nb * 2 + hi);
                     if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
                 }
             }
@@ -194,47 +228,58 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<MX, BF16>::T
     } else if (warp == 1) {
         // ---------------- MMA issuer (leader CTA only) ----------------
         if (rank == 0 && elect_one()) {
-            const uint32_t idesc = make_idesc_mx4(MX, 256u, 256u);
             int stage = 0;
             uint32_t phase = 0;
             bool ok = true;
             int it = 0;
+            int word = 0;       // of the scale ring
             long long seq = 0;  // k-blocks issued
-            for (int tile = cluster; tile < num_tiles && ok; tile += nclusters, ++it) {
-                // the previous tile's shared columns (and all of the tile before it) are drained
-                if (it > 0 && !mbar_wait(tempty, static_cast<uint32_t>(it - 1) & 1u, err)) { ok = false; break; }
-                tc_fence_after();
+            for (; it < units && ok; ++it) {
+                const uint32_t idesc = make_idesc_mx4(MX, 256u, pair_unit(whole, cluster, nclusters, it).half ? 128u : 256u);
                 const uint32_t d_tmem = tmem_base + ((it & 1) ? C::ACC1 : 0);
                 for (int kb = 0; kb < kblocks; ++kb, ++seq) {
                     if (!mbar_wait(&full[stage], phase, err)) { ok = false; break; }
-                    if (seq >= 2) {
-                        // the MMAs that read this scale slot two k-blocks ago are complete
+                    if (C::SF_WAIT && seq >= 2) {
+                        // The MMAs that read these scale words before are complete: the last of
+                        // them are the first two of two k-blocks ago.  (The order of one thread's
+                        // tcgen05 operations covers copy -> MMA, not MMA -> copy.)  Where the ring
+                        // holds every stage's words, the stage itself says so.
                         int st = stage - 2;
                         uint32_t ph = phase;
                         if (st < 0) { st += C::STAGES; ph ^= 1u; }
-                        if (!mbar_wait(&empty[st], ph, err)) { ok = false; break; }
+                        if (!mbar_wait(&mid[st], ph, err)) { ok = false; break; }
                     }
                     tc_fence_after();
-                    const uint32_t sfa = tmem_base + C::SF + static_cast<uint32_t>(seq & 1) * C::SF_SLOT;
-                    const uint32_t sfb = sfa + 4 * C::WORDS;
-                    const uint32_t sa = smem_u32(sSA + stage * C::SFA_BYTES), sb = smem_u32(sSB + stage * C::SFB_BYTES);
+                    // Descriptors once a stage, then their address fields (16-byte units) by
+                    // addition: built one by one they held the single issuing thread
+                    // behind the tensor pipe (250 -> 230 us at 8192 x 14336 x 4096).
+                    const uint64_t ga = smem_desc_rows16(smem_u32(sSA + stage * C::SFA_BYTES));
+                    const uint64_t gb = smem_desc_rows16(smem_u32(sSB + stage * C::SFB_BYTES));
+                    const uint64_t ad = smem_desc_sw128(smem_u32(sA + stage * C::A_BYTES), 16u, 1024u);
+                    const uint64_t bd = smem_desc_sw128(smem_u32(sB + stage * C::B_BYTES), 16u, 1024u);
+                    uint32_t sf[C::WORDS];
 #pragma unroll
                     for (int w = 0; w < C::WORDS; ++w) {
-                        tmem_cp_scales_pair(sfa + 4 * w, smem_desc_rows16(sa + 512 * w));
-                        tmem_cp_scales_pair(sfb + 8 * w, smem_desc_rows16(sb + 512 * w));
-                        tmem_cp_scales_pair(sfb + 8 * w + 4, smem_desc_rows16(sb + 512 * (C::WORDS + w)));
+                        sf[w] = tmem_base + C::SF + 12u * static_cast<uint32_t>(word);
+                        if (++word == C::RING) word = 0;
+                        tmem_cp_scales_pair(sf[w], ga + 32 * w);
+                        tmem_cp_scales_pair(sf[w] + 4, gb + 32 * w);
+                        tmem_cp_scales_pair(sf[w] + 8, gb + 32 * (C::WORDS + w));
                     }
-                    const uint32_t a_addr = smem_u32(sA + stage * C::A_BYTES);
-                    const uint32_t b_addr = smem_u32(sB + stage * C::B_BYTES);
+                    if (kb == 0 && it > 0) {
+                        // the previous tile's shared columns (and all of the tile before it) are drained
+                        if (!mbar_wait(tempty, static_cast<uint32_t>(it - 1) & 1u, err)) { ok = false; break; }
+                        tc_fence_after();
+                    }
                     const int mmas = min(4, (K - kb * BK + 63) / 64);
 #pragma unroll
                     for (int kk = 0; kk < 4; ++kk) {
-                        if (kk >= mmas) break;
-                        const uint64_t adesc = smem_desc_sw128(a_addr + 32u * kk, 16u, 1024u);
-                        const uint64_t bdesc = smem_desc_sw128(b_addr + 32u * kk, 16u, 1024u);
-                        const int w = MX ? kk / 2 : kk;
-                        const uint32_t id = idesc | (MX ? idesc_scale_ids(2u * (kk & 1)) : 0u);
-                        mma_mx4_pair<MX>(d_tmem, adesc, bdesc, id, sfa + 4 * w, sfb + 8 * w, (kb > 0 || kk > 0) ? 1u : 0u);
+                        if (kk < mmas) {
+                            const int w = MX ? kk / 2 : kk;
+                            const uint32_t id = idesc | (MX ? idesc_scale_ids(2u * (kk & 1)) : 0u);
+                            mma_mx4_pair<MX>(d_tmem, ad + 2 * kk, bd + 2 * kk, id, sf[w], sf[w] + 4, (kb > 0 || kk > 0) ? 1u : 0u);
+                        }
+                        if (C::SF_WAIT && kk == 1) tc_commit_pair_mc(&mid[stage], 0x1);
                     }
                     tc_commit_pair_mc(&empty[stage], 0x3);
                     if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
@@ -251,20 +296,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<MX, BF16>::T
         const uint32_t tempty_leader = mapa_shared(smem_u32(tempty), 0);
         uint8_t* slots = sEpi + (warp - 2) * 2 * C::SLOT;
         float* cols = reinterpret_cast<float*>(sCols + (warp - 2) * 256);  // 32 column scales, 32 biases
-        const bool has_cols = ep.col_scale || ep.bias;
+        const bool has_cols = ep.col_scale, has_bias = ep.bias;
         int it = 0;
         int chunk_seq = 0;
-        for (int tile = cluster; tile < num_tiles; tile += nclusters, ++it) {
+        for (; it < units; ++it) {
             const int acc = it & 1;
+            const PairUnit un = pair_unit(whole, cluster, nclusters, it);
             int mb, nb;
-            pair_tile(tile, m_tiles, n_tiles, mb, nb);
+            pair_tile(un.tile, m_tiles, n_tiles, mb, nb);
+            // the four chunks of a whole tile, or the two of a half in accumulator columns [0, 128)
+            const int nchunks = un.half ? 2 : 4;
+            const int half0 = un.half == 2 ? 128 : 0;
+            auto chunk = [&](int i) { return un.half ? 2 * g + i : chunk_of(acc, g, i); };
             const int row0 = mb * 256 + static_cast<int>(rank) * 128 + quarter * 32;
             const int row = row0 + lane;
-            const float rs = (ep.row_scale && row < M) ? __ldg(ep.row_scale + row) : 1.0f;
+            const float f1 = (ep.row_scale && row < M) ? __fmul_rn(ep.alpha, __ldg(ep.row_scale + row)) : ep.alpha;
+            const float2 f = make_float2(f1, f1);
             float cs[4], bs[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int c = min(nb * 256 + 32 * chunk_of(acc, g, i) + lane, N - 1);
+                const int c = min(nb * 256 + half0 + 32 * chunk(i) + lane, N - 1);
                 cs[i] = ep.col_scale ? __ldg(ep.col_scale + c) : 1.0f;
                 bs[i] = ep.bias ? __ldg(ep.bias + c) : -0.0f;
             }
@@ -273,8 +324,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<MX, BF16>::T
             tc_fence_after();
             const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + (acc ? C::ACC1 : 0);
             uint32_t r[2][32];
-            tmem_ld_32x32b_x32(taddr + 32 * chunk_of(acc, g, 0), r[0]);
-            tmem_ld_32x32b_x32(taddr + 32 * chunk_of(acc, g, 1), r[1]);
+            tmem_ld_32x32b_x32(taddr + 32 * chunk(0), r[0]);
+            tmem_ld_32x32b_x32(taddr + 32 * chunk(1), r[1]);
             tmem_ld_wait();
             after_tmem_ld(r[0]);
             after_tmem_ld(r[1]);
@@ -286,7 +337,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<MX, BF16>::T
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int col0 = nb * 256 + 32 * chunk_of(acc, g, i);
+                if (i >= nchunks) break;
+                const int col0 = nb * 256 + half0 + 32 * chunk(i);
                 uint32_t (&cur)[32] = r[i & 1];
                 if (i >= 2) {
                     tmem_ld_wait();
@@ -295,27 +347,31 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<MX, BF16>::T
                 if (col0 < N && row0 < M) {
                     uint8_t* slot = slots + (chunk_seq & 1) * C::SLOT;
                     if (ep.tma_out && lane == 0) bulk_wait_group_read<1>();  // the store two chunks ago has read this slot
-                    if (has_cols) {
-                        cols[lane] = cs[i];
-                        cols[32 + lane] = bs[i];
-                    }
+                    if (has_cols) cols[lane] = cs[i];
+                    if (has_bias) cols[32 + lane] = bs[i];
                     __syncwarp();
                     constexpr int PER = BF16 ? 8 : 4;  // outputs in 16 bytes
 #pragma unroll
                     for (int j = 0; j < 32 / PER; ++j) {
                         float v[PER];
 #pragma unroll
-                        for (int t = 0; t < PER; ++t) v[t] = __fmul_rn(__fmul_rn(__uint_as_float(cur[PER * j + t]), ep.alpha), rs);
-                        if (has_cols) {
-#pragma unroll
-                            for (int t = 0; t < PER; t += 4) {
+                        for (int t = 0; t < PER; t += 4) {
+                            float2 lo = mul2(make_float2(__uint_as_float(cur[PER * j + t]), __uint_as_float(cur[PER * j + t + 1])), f);
+                            float2 hi = mul2(make_float2(__uint_as_float(cur[PER * j + t + 2]), __uint_as_float(cur[PER * j + t + 3])), f);
+                            if (has_cols) {
                                 const float4 c4 = *reinterpret_cast<const float4*>(cols + PER * j + t);
-                                const float4 b4 = *reinterpret_cast<const float4*>(cols + 32 + PER * j + t);
-                                v[t] = __fadd_rn(__fmul_rn(v[t], c4.x), b4.x);
-                                v[t + 1] = __fadd_rn(__fmul_rn(v[t + 1], c4.y), b4.y);
-                                v[t + 2] = __fadd_rn(__fmul_rn(v[t + 2], c4.z), b4.z);
-                                v[t + 3] = __fadd_rn(__fmul_rn(v[t + 3], c4.w), b4.w);
+                                lo = mul2(lo, make_float2(c4.x, c4.y));
+                                hi = mul2(hi, make_float2(c4.z, c4.w));
                             }
+                            if (has_bias) {
+                                const float4 b4 = *reinterpret_cast<const float4*>(cols + 32 + PER * j + t);
+                                lo = add2(lo, make_float2(b4.x, b4.y));
+                                hi = add2(hi, make_float2(b4.z, b4.w));
+                            }
+                            v[t] = lo.x;
+                            v[t + 1] = lo.y;
+                            v[t + 2] = hi.x;
+                            v[t + 3] = hi.y;
                         }
                         if (BF16) {
                             // 64-byte rows, 16-byte unit j at j ^ ((row >> 1) & 3)
@@ -352,7 +408,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<MX, BF16>::T
                     }
                     ++chunk_seq;
                 }
-                if (i < 2) tmem_ld_32x32b_x32(taddr + 32 * chunk_of(acc, g, i + 2), cur);
+                if (i + 2 < nchunks) tmem_ld_32x32b_x32(taddr + 32 * chunk(i + 2), cur);
             }
         }
         if (lane == 0) bulk_wait_group_all();
@@ -386,7 +442,8 @@ struct DecodeCfg {
     static constexpr int STAGES = BUDGET / STAGE < 8 ? BUDGET / STAGE : 8;
     static constexpr int SMEM = 1024 + STAGES * STAGE + 2 * OUT_BYTES + BT * 4 + 256;
     static constexpr int SF = 128;           // tensor memory columns of the scales (accumulators below)
-    static constexpr int SF_SLOT = 8 * WORDS;
+    static constexpr int SF_SLOT = 8 * WORDS;  // a stage's scales
+    static constexpr int SF_SLOTS = 4;
     static constexpr int THREADS = 192;
 };
 
@@ -479,7 +536,7 @@ __global__ void __launch_bounds__(192, 1)
     pdl_wait();
     if (threadIdx.x >= 64 && threadIdx.x < 64 + BT) {
         const int t = threadIdx.x - 64;
-        sRs[t] = (ep.row_scale && t < M) ? __ldg(ep.row_scale + t) : 1.0f;
+        sRs[t] = (ep.row_scale && t < M) ? __fmul_rn(ep.alpha, __ldg(ep.row_scale + t)) : ep.alpha;
     }
     tc_fence_before();
     __syncthreads();
@@ -533,15 +590,15 @@ __global__ void __launch_bounds__(192, 1)
                 const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * BT);
                 for (long long kl = s0; kl < s1; ++kl, ++seq) {
                     if (!mbar_wait(&full[stage], phase, err)) { ok = false; break; }
-                    if (seq >= 2) {
-                        // the MMAs that read this scale slot two k-blocks ago are complete
-                        int st = stage - 2;
+                    if (seq >= C::SF_SLOTS) {
+                        // the MMAs that read this scale slot before are complete
+                        int st = stage - C::SF_SLOTS;
                         uint32_t ph = phase;
                         if (st < 0) { st += C::STAGES; ph ^= 1u; }
                         if (!mbar_wait(&empty[st], ph, err)) { ok = false; break; }
                     }
                     tc_fence_after();
-                    const uint32_t sfw = tmem_base + C::SF + static_cast<uint32_t>(seq & 1) * C::SF_SLOT;
+                    const uint32_t sfw = tmem_base + C::SF + static_cast<uint32_t>(seq % C::SF_SLOTS) * C::SF_SLOT;
                     const uint32_t sfx = sfw + 4 * C::WORDS;
                     const uint32_t gw = smem_u32(sSW + stage * C::SF_BYTES), gx = smem_u32(sSX + stage * C::SF_BYTES);
 #pragma unroll
@@ -631,7 +688,7 @@ __global__ void __launch_bounds__(192, 1)
                 }
                 float v[16];
 #pragma unroll
-                for (int j = 0; j < 16; ++j) v[j] = mx_epi(__uint_as_float(r[j]), ep.alpha, sRs[c + j], cs, bs);
+                for (int j = 0; j < 16; ++j) v[j] = mx_epi(__uint_as_float(r[j]), sRs[c + j], cs, bs);
                 // [row of A][row of B] in the output type
                 if (ep.out_bf16) {
                     uint16_t* o = reinterpret_cast<uint16_t*>(sOut) + c * 128 + nl;
@@ -747,10 +804,11 @@ nq_status_t launch_pair(const Operands& o, const MxEpi& ep, const DeviceInfo& di
     using C = PairCfg<MX, BF16>;
     const uint64_t pitch = mx4_pitch(o.k);
     const int words = mx4_words(o.k, MX ? 32 : 16);
-    CUtensorMap ma, mb, msa, msb, mc;
+    CUtensorMap ma, mb, mbh, msa, msb, mc;
     std::memset(&mc, 0, sizeof(mc));
     nq_status_t st = make_map(&ma, o.a, pitch, o.m, pitch, BKB, 128);
     if (st == NQ_SUCCESS) st = make_map(&mb, o.b, pitch, o.n, pitch, BKB, 128);
+    if (st == NQ_SUCCESS) st = make_map(&mbh, o.b, pitch, o.n, pitch, BKB, 64);
     if (st == NQ_SUCCESS) st = make_scale_map(&msa, o.sa, o.m, words, C::WORDS, 1);
     if (st == NQ_SUCCESS) st = make_scale_map(&msb, o.sb, o.n, words, C::WORDS, 2);
     if (st == NQ_SUCCESS && ep.tma_out) st = make_out_map(&mc, ep, o.m, o.n, 32, 32, true);
@@ -773,9 +831,15 @@ nq_status_t launch_pair(const Operands& o, const MxEpi& ep, const DeviceInfo& di
         max_clusters[di.device & 63].store(resident, std::memory_order_relaxed);
     }
     const long long tiles = static_cast<long long>((o.m + 255) / 256) * ((o.n + 255) / 256);
-    const int clusters = static_cast<int>(std::max<long long>(1, std::min<long long>(tiles, resident)));
-    return cuda_status(launch_pdl(kern, dim3(2 * clusters), dim3(C::THREADS), C::SMEM, s, ma, mb, msa, msb, mc, o.m, o.n, o.k, ep,
-                                  device_error_word()),
+    if (tiles > (1 << 30)) return fail(NQ_ERROR_UNSUPPORTED, "nq_gemm_mx4: more than 2^30 output tiles");
+    // A last wave that fills at most half the clusters runs as half tiles: the
+    // tail takes half a tile's time (4096^3, 3.46 waves: 28.9 -> 27.4 us).
+    const int rest = static_cast<int>(tiles % resident);
+    const int whole = static_cast<int>(2 * rest <= resident ? tiles - rest : tiles);
+    const long long units = whole < tiles ? std::max<long long>(std::min<long long>(whole, resident), 2 * rest) : tiles;
+    const int clusters = static_cast<int>(std::max<long long>(1, std::min<long long>(units, resident)));
+    return cuda_status(launch_pdl(kern, dim3(2 * clusters), dim3(C::THREADS), C::SMEM, s, ma, mb, mbh, msa, msb, mc, o.m, o.n, o.k,
+                                  whole, ep, device_error_word()),
                        "nq_gemm_mx4 (CTA pair)");
 }
 
