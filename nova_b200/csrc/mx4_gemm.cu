@@ -422,14 +422,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<MX, BF16>::T
     }
 }
 
-// ---------------- up to 64 rows: swapped operands, shared-out k-blocks ----------------
-// The k-blocks of all 128-row slices of B, in slice order, are cut into one
-// contiguous range a CTA.  The CTA that holds a slice's first k-block finishes
-// it; a CTA that starts inside a slice parks its accumulators in its workspace
-// row and raises its flag, and the owner adds the parts in range order: no
-// atomics, the same sums every time.  Ranges go to the CTAs in reverse, so an
-// owner waits for CTAs of lower index only: those are placed before it, and a
-// grid that shares the GPU with another one still finishes.
+// ---------------- up to 64 rows: swapped operands ----------------
+// Units of 128 rows of B (the MMA's M side), dealt whole to the CTAs, or with
+// `split` their k-blocks shared out: the k-blocks of all units in order are cut into one contiguous range a
+// CTA.  The CTA that holds a unit's first k-block finishes it; a CTA that starts
+// inside a unit parks its accumulators in its workspace row and raises its
+// flag, and the owner adds the parts in range order: no atomics, the same sums
+// every time.  Ranges go to the CTAs in reverse, so an owner waits for CTAs of
+// lower index only: those are placed before it, and a grid that shares the GPU
+// with another one still finishes.
 template <bool MX, int BT>
 struct DecodeCfg {
     static constexpr int WORDS = MX ? 2 : 4;
@@ -442,8 +443,8 @@ struct DecodeCfg {
     static constexpr int STAGES = BUDGET / STAGE < 8 ? BUDGET / STAGE : 8;
     static constexpr int SMEM = 1024 + STAGES * STAGE + 2 * OUT_BYTES + BT * 4 + 256;
     static constexpr int SF = 128;           // tensor memory columns of the scales (accumulators below)
-    static constexpr int SF_SLOT = 8 * WORDS;  // a stage's scales
-    static constexpr int SF_SLOTS = 4;
+    static constexpr int SF_SLOT = 8 * WORDS;  // a slot for every stage's scales
+    static_assert(SF + STAGES * SF_SLOT <= 512, "tensor memory");
     static constexpr int THREADS = 192;
 };
 
@@ -466,7 +467,7 @@ template <bool MX, int BT>
 __global__ void __launch_bounds__(192, 1)
     k_mx4_decode(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
                  const __grid_constant__ CUtensorMap tmSW, const __grid_constant__ CUtensorMap tmSX,
-                 const __grid_constant__ CUtensorMap tmO, int M, int N, int K, MxEpi ep, uint32_t* ws, uint32_t* flags,
+                 const __grid_constant__ CUtensorMap tmO, int M, int N, int K, int split, MxEpi ep, uint32_t* ws, uint32_t* flags,
                  uint32_t* err) {
     using C = DecodeCfg<MX, BT>;
     extern __shared__ uint8_t smem_raw[];
@@ -490,16 +491,31 @@ __global__ void __launch_bounds__(192, 1)
     const int lane = threadIdx.x & 31;
     const int G = gridDim.x;
     const int kblocks = (K + BK - 1) / BK;
-    const long long total = static_cast<long long>((N + 127) / 128) * kblocks;
-    const int cta = G - 1 - static_cast<int>(blockIdx.x);  // this CTA's range
-    const long long b0 = range_begin(total, cta, G);
-    const long long b1 = range_begin(total, cta + 1, G);
-    // this CTA's last segment: does it own a slice whose rest is one later range's?
-    const int last_slice = static_cast<int>((b1 - 1) / kblocks);
-    const long long last_s0 = max(b0, static_cast<long long>(last_slice) * kblocks);
-    int lc_first, lc_last;
-    later_ranges(total, cta, G, b1, static_cast<long long>(last_slice + 1) * kblocks, &lc_first, &lc_last);
-    const bool last_fetch = (last_s0 % kblocks) == 0 && lc_last == lc_first;
+    const int unit_n = (N + 127) / 128;
+    const long long total = static_cast<long long>(unit_n) * kblocks;
+    const int cta = G - 1 - static_cast<int>(blockIdx.x);  // this CTA's range (split)
+    // work positions: k-blocks [b0, b1) of all units in order, or units b0, b0 + G, ... below b1
+    const long long b0 = split ? range_begin(total, cta, G) : blockIdx.x;
+    const long long b1 = split ? range_begin(total, cta + 1, G) : unit_n;
+    struct Seg {
+        int unit, kb0, kb1;
+        long long next;
+    };
+    auto segment = [&](long long pos) {
+        if (!split) return Seg{static_cast<int>(pos), 0, kblocks, pos + G};
+        const int unit = static_cast<int>(pos / kblocks);
+        const long long u0 = static_cast<long long>(unit) * kblocks;
+        const long long next = min(b1, u0 + kblocks);
+        return Seg{unit, static_cast<int>(pos - u0), static_cast<int>(next - u0), next};
+    };
+    // split: does this CTA's last segment own a unit whose rest is one later range's?
+    int lc_first = 1, lc_last = 0;
+    bool last_fetch = false;
+    if (split) {
+        const int last = static_cast<int>((b1 - 1) / kblocks);
+        later_ranges(total, cta, G, b1, static_cast<long long>(last + 1) * kblocks, &lc_first, &lc_last);
+        last_fetch = b0 <= static_cast<long long>(last) * kblocks && lc_last == lc_first;
+    }
 
     // Up to pdl_wait() nothing touches memory that an earlier kernel may write
     // (the prefetch only fills L2, which is coherent).
@@ -523,14 +539,14 @@ __global__ void __launch_bounds__(192, 1)
         tma_prefetch_desc(&tmSW);
         tma_prefetch_desc(&tmSX);
         if (ep.tma_out) tma_prefetch_desc(&tmO);
-        for (long long kl = b0; kl < b1 && kl < b0 + C::STAGES; ++kl) {
-            const int slice = static_cast<int>(kl / kblocks), kb = static_cast<int>(kl % kblocks);
-            tma_prefetch_l2_2d(&tmW, kb * BKB, slice * 128);
-            tma_prefetch_l2_2d(&tmSW, kb * C::WORDS * 64, slice);
+        const Seg g = segment(b0);
+        for (int kb = g.kb0; kb < g.kb1 && kb < g.kb0 + C::STAGES; ++kb) {
+            tma_prefetch_l2_2d(&tmW, kb * BKB, g.unit * 128);
+            tma_prefetch_l2_2d(&tmSW, kb * C::WORDS * 64, g.unit);
         }
     }
     if (warp == 1) {
-        tmem_alloc(tmem_slot, 256);
+        tmem_alloc(tmem_slot, 512);
         tmem_relinquish();
     }
     pdl_wait();
@@ -548,15 +564,18 @@ __global__ void __launch_bounds__(192, 1)
             int stage = 0;
             uint32_t phase = 0;
             bool ok = true;
-            for (long long kl = b0; kl < b1; ++kl) {
-                const int slice = static_cast<int>(kl / kblocks), kb = static_cast<int>(kl % kblocks);
-                if (!mbar_wait(&empty[stage], phase ^ 1u, err)) { ok = false; break; }
-                mbar_arrive_expect_tx(&full[stage], C::STAGE);
-                tma_load_2d(sW + stage * C::W_BYTES, &tmW, &full[stage], kb * BKB, slice * 128);
-                tma_load_2d(sSW + stage * C::SF_BYTES, &tmSW, &full[stage], kb * C::WORDS * 64, slice);
-                tma_load_2d(sX + stage * C::X_BYTES, &tmX, &full[stage], kb * BKB, 0);
-                tma_load_2d(sSX + stage * C::SF_BYTES, &tmSX, &full[stage], kb * C::WORDS * 64, 0);
-                if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
+            for (long long pos = b0; pos < b1 && ok;) {
+                const Seg g = segment(pos);
+                pos = g.next;
+                for (int kb = g.kb0; kb < g.kb1; ++kb) {
+                    if (!mbar_wait(&empty[stage], phase ^ 1u, err)) { ok = false; break; }
+                    mbar_arrive_expect_tx(&full[stage], C::STAGE);
+                    tma_load_2d(sW + stage * C::W_BYTES, &tmW, &full[stage], kb * BKB, g.unit * 128);
+                    tma_load_2d(sSW + stage * C::SF_BYTES, &tmSW, &full[stage], kb * C::WORDS * 64, g.unit);
+                    tma_load_2d(sX + stage * C::X_BYTES, &tmX, &full[stage], kb * BKB, 0);
+                    tma_load_2d(sSX + stage * C::SF_BYTES, &tmSX, &full[stage], kb * C::WORDS * 64, 0);
+                    if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
+                }
             }
             if (!ok) {
                 // the copies in flight land before the CTA ends: the stages are freed by the MMAs that read them
@@ -579,50 +598,41 @@ __global__ void __launch_bounds__(192, 1)
             int stage = 0;
             uint32_t phase = 0;
             int seg = 0;
-            long long seq = 0;
             bool ok = true;
-            for (long long s0 = b0; s0 < b1 && ok; ++seg) {
-                const int slice = static_cast<int>(s0 / kblocks);
-                const long long s1 = min(b1, static_cast<long long>(slice + 1) * kblocks);
+            for (long long pos = b0; pos < b1 && ok; ++seg) {
+                const Seg g = segment(pos);
+                pos = g.next;
                 const int acc = seg & 1;
                 if (!mbar_wait(&tempty[acc], ((static_cast<uint32_t>(seg) >> 1) & 1u) ^ 1u, err)) { ok = false; break; }
                 tc_fence_after();
                 const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * BT);
-                for (long long kl = s0; kl < s1; ++kl, ++seq) {
+                for (int kb = g.kb0; kb < g.kb1; ++kb) {
                     if (!mbar_wait(&full[stage], phase, err)) { ok = false; break; }
-                    if (seq >= C::SF_SLOTS) {
-                        // the MMAs that read this scale slot before are complete
-                        int st = stage - C::SF_SLOTS;
-                        uint32_t ph = phase;
-                        if (st < 0) { st += C::STAGES; ph ^= 1u; }
-                        if (!mbar_wait(&empty[st], ph, err)) { ok = false; break; }
-                    }
                     tc_fence_after();
-                    const uint32_t sfw = tmem_base + C::SF + static_cast<uint32_t>(seq % C::SF_SLOTS) * C::SF_SLOT;
+                    // (the MMAs that read this slot before have freed the stage)
+                    const uint32_t sfw = tmem_base + C::SF + static_cast<uint32_t>(stage) * C::SF_SLOT;
                     const uint32_t sfx = sfw + 4 * C::WORDS;
-                    const uint32_t gw = smem_u32(sSW + stage * C::SF_BYTES), gx = smem_u32(sSX + stage * C::SF_BYTES);
+                    const uint64_t gw = smem_desc_rows16(smem_u32(sSW + stage * C::SF_BYTES));
+                    const uint64_t gx = smem_desc_rows16(smem_u32(sSX + stage * C::SF_BYTES));
+                    const uint64_t ad = smem_desc_sw128(smem_u32(sW + stage * C::W_BYTES), 16u, 1024u);
+                    const uint64_t bd = smem_desc_sw128(smem_u32(sX + stage * C::X_BYTES), 16u, 1024u);
 #pragma unroll
                     for (int w = 0; w < C::WORDS; ++w) {
-                        tmem_cp_scales(sfw + 4 * w, smem_desc_rows16(gw + 512 * w));
-                        tmem_cp_scales(sfx + 4 * w, smem_desc_rows16(gx + 512 * w));
+                        tmem_cp_scales(sfw + 4 * w, gw + 32 * w);
+                        tmem_cp_scales(sfx + 4 * w, gx + 32 * w);
                     }
-                    const uint32_t a_addr = smem_u32(sW + stage * C::W_BYTES);
-                    const uint32_t b_addr = smem_u32(sX + stage * C::X_BYTES);
-                    const int mmas = min(4, (K - static_cast<int>(kl % kblocks) * BK + 63) / 64);
+                    const int mmas = min(4, (K - kb * BK + 63) / 64);
 #pragma unroll
                     for (int kk = 0; kk < 4; ++kk) {
                         if (kk >= mmas) break;
-                        const uint64_t adesc = smem_desc_sw128(a_addr + 32u * kk, 16u, 1024u);
-                        const uint64_t bdesc = smem_desc_sw128(b_addr + 32u * kk, 16u, 1024u);
                         const int w = MX ? kk / 2 : kk;
                         const uint32_t id = idesc | (MX ? idesc_scale_ids(2u * (kk & 1)) : 0u);
-                        mma_mx4<MX>(d_tmem, adesc, bdesc, id, sfw + 4 * w, sfx + 4 * w, (kl > s0 || kk > 0) ? 1u : 0u);
+                        mma_mx4<MX>(d_tmem, ad + 2 * kk, bd + 2 * kk, id, sfw + 4 * w, sfx + 4 * w, (kb > g.kb0 || kk > 0) ? 1u : 0u);
                     }
                     tc_commit(&empty[stage]);
                     if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
                 }
                 if (ok) tc_commit(&tfull[acc]);
-                s0 = s1;
             }
             tc_commit(done);
             mbar_wait(done, 0, err);
@@ -637,22 +647,23 @@ __global__ void __launch_bounds__(192, 1)
         bool failed = false;
         int seg = 0;
         uint32_t* sOut32 = reinterpret_cast<uint32_t*>(sOut);
-        for (long long s0 = b0; s0 < b1; ++seg) {
-            const int slice = static_cast<int>(s0 / kblocks);
-            const long long slice_end = static_cast<long long>(slice + 1) * kblocks;
-            const long long s1 = min(b1, slice_end);
-            const bool head = (s0 % kblocks) == 0;  // this CTA holds the slice's first k-block
+        for (long long pos = b0; pos < b1; ++seg) {
+            const Seg g = segment(pos);
+            pos = g.next;
+            const bool head = g.kb0 == 0;  // this CTA holds the unit's first k-block
             const int acc = seg & 1;
             const uint32_t tpar = (static_cast<uint32_t>(seg) >> 1) & 1u;
             const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(acc * BT);
             int c_first = 1, c_last = 0;
-            if (head) later_ranges(total, cta, G, s1, slice_end, &c_first, &c_last);
-            const bool split = c_last >= c_first;
-            const bool fetched = split && s1 == b1 && last_fetch;  // the producer bulk-loads the part
-            const int n = slice * 128 + nl;
-            const float cs = head && ep.col_scale && n < N ? __ldg(ep.col_scale + n) : 1.0f;
-            const float bs = head && ep.bias && n < N ? __ldg(ep.bias + n) : -0.0f;
-            if (split && !fetched) {
+            if (split && head)
+                later_ranges(total, cta, G, g.next, static_cast<long long>(g.unit + 1) * kblocks, &c_first, &c_last);
+            const bool parts = c_last >= c_first;
+            const bool fetched = parts && g.next == b1 && last_fetch;  // the producer bulk-loads the part
+            const int n = g.unit * 128 + nl;
+            const bool mine = n < N;
+            const float cs = head && ep.col_scale && mine ? __ldg(ep.col_scale + n) : 1.0f;
+            const float bs = head && ep.bias && mine ? __ldg(ep.bias + n) : -0.0f;
+            if (parts && !fetched) {
                 if (lane == 0)
                     for (int c = c_first; c <= c_last; ++c) wait_flag_geq(flags + c * 4, 1u, err);
                 __syncwarp();
@@ -663,44 +674,43 @@ __global__ void __launch_bounds__(192, 1)
             // the previous bulk store has read sOut, and every warp has passed its
             // flag wait (so the flags can be cleared below)
             named_bar_sync(1, 128);
-#pragma unroll 1
-            for (int c = 0; c < BT; c += 16) {
-                uint32_t r[16];
-                tmem_ld_32x32b_x16(taddr + c, r);
-                tmem_ld_wait();
-                after_tmem_ld(r);
-                if (!head) {
+            uint32_t r[BT];  // this thread's row of B against every row of A
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) sOut32[(c + j) * 128 + nl] = r[j];
-                    continue;
-                }
+            for (int c = 0; c < BT; c += 16) tmem_ld_32x32b_x16(taddr + c, *reinterpret_cast<uint32_t(*)[16]>(r + c));
+            tmem_ld_wait();
+            after_tmem_ld(r);
+            if (!head) {
+#pragma unroll
+                for (int j = 0; j < BT; ++j) sOut32[j * 128 + nl] = r[j];
+            } else {
                 if (fetched) {
 #pragma unroll
-                    for (int j = 0; j < 16; ++j)
-                        r[j] = __float_as_uint(__fadd_rn(__uint_as_float(r[j]), __uint_as_float(sPart[(c + j) * 128 + nl])));
-                } else if (split) {
+                    for (int j = 0; j < BT; ++j)
+                        r[j] = __float_as_uint(__fadd_rn(__uint_as_float(r[j]), __uint_as_float(sPart[j * 128 + nl])));
+                } else if (parts) {
+                    // a whole part's loads in flight at once
                     for (int cc = c_first; cc <= c_last; ++cc) {
-                        const uint32_t* part = ws + static_cast<size_t>(cc) * BT * 128;
+                        const uint32_t* part = ws + static_cast<size_t>(cc) * BT * 128 + nl;
+                        uint32_t q[BT];
 #pragma unroll
-                        for (int j = 0; j < 16; ++j)
-                            r[j] = __float_as_uint(__fadd_rn(__uint_as_float(r[j]), __uint_as_float(__ldcg(part + (c + j) * 128 + nl))));
+                        for (int j = 0; j < BT; ++j) q[j] = __ldcg(part + j * 128);
+#pragma unroll
+                        for (int j = 0; j < BT; ++j) r[j] = __float_as_uint(__fadd_rn(__uint_as_float(r[j]), __uint_as_float(q[j])));
                     }
                 }
-                float v[16];
-#pragma unroll
-                for (int j = 0; j < 16; ++j) v[j] = mx_epi(__uint_as_float(r[j]), sRs[c + j], cs, bs);
                 // [row of A][row of B] in the output type
-                if (ep.out_bf16) {
-                    uint16_t* o = reinterpret_cast<uint16_t*>(sOut) + c * 128 + nl;
 #pragma unroll
-                    for (int j = 0; j < 16; j += 2) {
-                        const uint32_t p2 = f32x2_to_bf16x2(v[j], v[j + 1]);
-                        o[j * 128] = static_cast<uint16_t>(p2);
-                        o[(j + 1) * 128] = static_cast<uint16_t>(p2 >> 16);
+                for (int j = 0; j < BT; j += 2) {
+                    const float v0 = mx_epi(__uint_as_float(r[j]), sRs[j], cs, bs);
+                    const float v1 = mx_epi(__uint_as_float(r[j + 1]), sRs[j + 1], cs, bs);
+                    if (ep.out_bf16) {
+                        const uint32_t p2 = f32x2_to_bf16x2(v0, v1);
+                        reinterpret_cast<uint16_t*>(sOut)[j * 128 + nl] = static_cast<uint16_t>(p2);
+                        reinterpret_cast<uint16_t*>(sOut)[(j + 1) * 128 + nl] = static_cast<uint16_t>(p2 >> 16);
+                    } else {
+                        sOut32[j * 128 + nl] = __float_as_uint(v0);
+                        sOut32[(j + 1) * 128 + nl] = __float_as_uint(v1);
                     }
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) sOut32[(c + j) * 128 + nl] = __float_as_uint(v[j]);
                 }
             }
             tc_fence_before();
@@ -720,11 +730,11 @@ __global__ void __launch_bounds__(192, 1)
             } else {
                 if (ep.tma_out) {
                     if (issuer) {
-                        tma_store_2d(&tmO, sOut, slice * 128, 0);  // clips rows >= M and columns >= N
+                        tma_store_2d(&tmO, sOut, g.unit * 128, 0);  // clips rows >= M and columns >= N
                         bulk_commit_group();
                         bulk_wait_group_read<0>();
                     }
-                } else if (n < N) {
+                } else if (mine) {
                     for (int t = 0; t < M; ++t) {
                         const size_t at = static_cast<size_t>(t) * N + n;
                         if (ep.out_bf16) static_cast<uint16_t*>(ep.out)[at] = reinterpret_cast<uint16_t*>(sOut)[t * 128 + nl];
@@ -736,7 +746,6 @@ __global__ void __launch_bounds__(192, 1)
                 if (issuer)
                     for (int cc = c_first; cc <= c_last; ++cc) flags[cc * 4] = 0u;
             }
-            s0 = s1;
         }
         if (issuer) bulk_wait_group<0>();
     }
@@ -744,7 +753,7 @@ __global__ void __launch_bounds__(192, 1)
     __syncthreads();
     if (warp == 1) {
         tc_fence_after();
-        tmem_dealloc(tmem_base, 256);
+        tmem_dealloc(tmem_base, 512);
     }
 }
 
@@ -844,7 +853,7 @@ nq_status_t launch_pair(const Operands& o, const MxEpi& ep, const DeviceInfo& di
 }
 
 template <bool MX, int BT>
-nq_status_t launch_decode(const Operands& o, const MxEpi& ep, const DeviceInfo& di, cudaStream_t s) {
+nq_status_t launch_decode(const Operands& o, const MxEpi& ep, int split, int grid, const DeviceInfo& di, cudaStream_t s) {
     using C = DecodeCfg<MX, BT>;
     const uint64_t pitch = mx4_pitch(o.k);
     const int words = mx4_words(o.k, MX ? 32 : 16);
@@ -860,36 +869,77 @@ nq_status_t launch_decode(const Operands& o, const MxEpi& ep, const DeviceInfo& 
     static std::atomic<uint64_t> attr_set{0};
     st = smem_attr(kern, C::SMEM, di.device, &attr_set);
     if (st != NQ_SUCCESS) return st;
-    const long long total = static_cast<long long>((o.n + 127) / 128) * ((o.k + BK - 1) / BK);
-    const int grid = static_cast<int>(std::max<long long>(1, std::min<long long>(total, di.sm_count)));
-    // per CTA one parked part and one flag (stride 4) of the stream's flag words,
-    // which every launch leaves cleared
-    const size_t ws_bytes = static_cast<size_t>(grid) * C::OUT_BYTES;
-    const size_t fl_bytes = static_cast<size_t>(grid) * 4 * 4;
     uint32_t* flags = nullptr;
-    st = stream_flags(&flags, grid * 4, s);
-    if (st != NQ_SUCCESS) return st;
     void* ws = nullptr;
-    st = scratch_alloc(&ws, ws_bytes + (flags ? 0 : fl_bytes), s);
-    if (st != NQ_SUCCESS) return st;
     cudaError_t e = cudaSuccess;
-    if (!flags) {
-        // inside a graph capture: flags of this launch, cleared by a memset node
-        flags = reinterpret_cast<uint32_t*>(static_cast<char*>(ws) + ws_bytes);
-        e = cudaMemsetAsync(flags, 0, fl_bytes, s);
+    if (split) {
+        // per CTA one parked part and one flag (stride 4) of the stream's flag words,
+        // which every launch leaves cleared
+        const size_t ws_bytes = static_cast<size_t>(grid) * C::OUT_BYTES;
+        const size_t fl_bytes = static_cast<size_t>(grid) * 4 * 4;
+        st = stream_flags(&flags, grid * 4, s);
+        if (st != NQ_SUCCESS) return st;
+        st = scratch_alloc(&ws, ws_bytes + (flags ? 0 : fl_bytes), s);
+        if (st != NQ_SUCCESS) return st;
+        if (!flags) {
+            // inside a graph capture: flags of this launch, cleared by a memset node
+            flags = reinterpret_cast<uint32_t*>(static_cast<char*>(ws) + ws_bytes);
+            e = cudaMemsetAsync(flags, 0, fl_bytes, s);
+        }
     }
     if (e == cudaSuccess)
-        e = launch_pdl(kern, dim3(grid), dim3(C::THREADS), C::SMEM, s, mw, mx, msw, msx, mo, o.m, o.n, o.k, ep,
+        e = launch_pdl(kern, dim3(grid), dim3(C::THREADS), C::SMEM, s, mw, mx, msw, msx, mo, o.m, o.n, o.k, split, ep,
                        static_cast<uint32_t*>(ws), flags, device_error_word());
     scratch_free(ws, s);
     return cuda_status(e, "nq_gemm_mx4 (few rows)");
 }
 
 template <bool MX>
+nq_status_t decode(const Operands& o, const MxEpi& ep, int split, int grid, const DeviceInfo& di, cudaStream_t s) {
+    if (o.m <= 16) return launch_decode<MX, 16>(o, ep, split, grid, di, s);
+    if (o.m <= 32) return launch_decode<MX, 32>(o, ep, split, grid, di, s);
+    return launch_decode<MX, 64>(o, ep, split, grid, di, s);
+}
+
+// Whole units or shared-out k-blocks, and on how many CTAs: the smallest of a few
+// estimates (us).  A k-block takes a CTA 0.27 us (its MMAs and copies) or its
+// share of HBM, whichever is longer (fewer CTAs reach two thirds of it); whole units cost 2.9 us besides, shared-out
+// ones 4.2 us and a part's way through memory for each CTA of a unit (0.45 us at 16
+// rows, 1 us at 64).  Measured, NVFP4, whole / shared out: 16 x 28672 x 8192 26.7 /
+// 24.7, 1 x 4096 x 4096 7.4 / 7.6, 4 x 4096 x 28672 32.9 / 17.0, 16 x 5000 x 3000
+// 6.4 / 7.5.
+struct DecodePlan {
+    int split, grid;
+};
+DecodePlan plan_decode(const Operands& o, bool mx, int sms) {
+    const long long units = (static_cast<long long>(o.n) + 127) / 128;
+    const long long kblocks = (o.k + BK - 1) / BK;
+    const double share = (mx ? 17.4e3 : 18.4e3) * sms / 6.5e6;  // us a k-block with every SM streaming
+    auto t_kb = [&](double active) { return std::max(0.27, std::min(share, 1.5 * share * active / sms)); };
+    DecodePlan best{0, static_cast<int>(std::min<long long>(units, sms))};
+    const long long rest = units % sms;
+    double best_us = 2.9 + static_cast<double>(kblocks) *
+                               (static_cast<double>(units / sms) * t_kb(sms) + (rest ? t_kb(static_cast<double>(rest)) : 0.0));
+    const double part_us = o.m <= 16 ? 0.45 : (o.m <= 32 ? 0.6 : 1.0);
+    auto offer = [&](long long grid, double parts) {
+        if (grid < 1 || grid > units * kblocks) return;
+        const double us = 4.2 + parts * part_us + static_cast<double>(units * kblocks) / grid * t_kb(static_cast<double>(grid));
+        if (us < best_us) {
+            best_us = us;
+            best = DecodePlan{1, static_cast<int>(grid)};
+        }
+    };
+    offer(sms, static_cast<double>(sms) / units + 1.0);
+    for (long long p = 2; p <= kblocks && units * p <= sms; ++p) offer(units * p, static_cast<double>(p));
+    return best;
+}
+
+template <bool MX>
 nq_status_t launch_gemm(const Operands& o, const MxEpi& ep, const DeviceInfo& di, cudaStream_t s) {
-    if (o.m <= 16) return launch_decode<MX, 16>(o, ep, di, s);
-    if (o.m <= 32) return launch_decode<MX, 32>(o, ep, di, s);
-    if (o.m <= 64) return launch_decode<MX, 64>(o, ep, di, s);
+    if (o.m <= 64) {
+        const DecodePlan p = plan_decode(o, MX, di.sm_count);
+        return decode<MX>(o, ep, p.split, p.grid, di, s);
+    }
     return ep.out_bf16 ? launch_pair<MX, true>(o, ep, di, s) : launch_pair<MX, false>(o, ep, di, s);
 }
 
