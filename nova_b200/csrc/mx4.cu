@@ -49,25 +49,19 @@ __global__ void __launch_bounds__(kThreads) k_mx4_quant_wide(const In* __restric
     for (long long rl = blockIdx.x; rl < rows; rl += gridDim.x, parity ^= 1) {
         const int row = static_cast<int>(rl);
         const In* x = src + row * ld;
-        float level = 0.0f;
-        bool ok = true;
+        NvRow nr{};
         if (F == kNVFP4) {
             uint32_t m = 0;
-            for (int v = threadIdx.x; v - lane < nvec; v += kThreads) {
-                float f[8];
-                unpack8<In>(load_vec<In, VEC>(x, v, cols, buf), f);
-                m = max(m, amax_bits8(f));
-            }
+            for (int v = threadIdx.x; v - lane < nvec; v += kThreads)
+                m = max(m, amax_bits_raw<In>(load_vec<In, VEC>(x, v, cols, buf)));
             m = block_umax(m, parity);
-            ok = m < kInfBits;
-            level = nv_row_level(m);
-            if (threadIdx.x == 0) rscales[row] = nv_row_scale(m, level);
+            nr = nv_row(m);
+            if (threadIdx.x == 0) rscales[row] = nv_row_scale(m, nr.level);
         }
         for (int v = threadIdx.x; v - lane < nstep; v += kThreads) {
-            float f[8];
-            unpack8<In>(load_vec<In, VEC>(x, v, cols, buf), f);
+            const Raw8<In> r = load_vec<In, VEC>(x, v, cols, buf);
             uint32_t byte;
-            const uint32_t c = mx4_encode<F>(f, level, ok, &byte);
+            const uint32_t c = mx4_encode<F>(unpack8<In>(r), amax_bits_raw<In>(r), nr, &byte);
             mx4_store<F>(codes + row * mx4_pitch(cols), bscales, row, v, pitch_words, words, c, byte);
         }
     }
@@ -93,27 +87,22 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) k_mx4_quant(const In* __res
         const int row = static_cast<int>(rl);
         Raw8<In> x[NV];
         load_vecs<In, VEC, NV>(x, src + row * ld, t0, width, cols, buf);
-        float level = 0.0f;
-        bool ok = true;
-        if (F == kNVFP4) {
-            uint32_t m = 0;
+        uint32_t am[NV];
 #pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                float f[8];
-                unpack8<In>(x[i], f);
-                m = max(m, amax_bits8(f));
-            }
+        for (int i = 0; i < NV; ++i) am[i] = amax_bits_raw<In>(x[i]);
+        NvRow nr{};
+        if (F == kNVFP4) {
+            uint32_t m = am[0];
+#pragma unroll
+            for (int i = 1; i < NV; ++i) m = max(m, am[i]);
             m = WARP ? __reduce_max_sync(0xffffffffu, m) : block_umax(m, parity);
-            ok = m < kInfBits;
-            level = nv_row_level(m);
-            if (t0 == 0) rscales[row] = nv_row_scale(m, level);
+            nr = nv_row(m);
+            if (t0 == 0) rscales[row] = nv_row_scale(m, nr.level);
         }
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            float f[8];
-            unpack8<In>(x[i], f);
             uint32_t byte;
-            const uint32_t c = mx4_encode<F>(f, level, ok, &byte);
+            const uint32_t c = mx4_encode<F>(unpack8<In>(x[i]), am[i], nr, &byte);
             mx4_store<F>(codes + row * mx4_pitch(cols), bscales, row, t0 + i * width, pitch_words, words, c, byte);
         }
     }
@@ -148,11 +137,14 @@ __global__ void __launch_bounds__(kThreads) k_mx4_dequant(const uint8_t* __restr
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                float f[8];
+                F8 f;
                 e2m1_decode8(c[i], f);
                 const float sv = mx4_scale_value(F, s[i]);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) f[e] = __fmul_rn(__fmul_rn(f[e], sv), g);
+                for (int j = 0; j < 4; ++j) {
+                    f.p[j] = mul2(f.p[j], both(sv));
+                    if (rscales) f.p[j] = mul2(f.p[j], both(g));
+                }
                 store_vec<T, VEC>(out, v0 + i * width, cols, pack8<T>(f), buf);
             }
         }

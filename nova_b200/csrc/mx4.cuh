@@ -43,8 +43,31 @@ __host__ __device__ __forceinline__ size_t mx4_scale_offset(int row, int word, i
     return (static_cast<size_t>(row >> 7) * words + word) * 512 + (row & 31) * 16 + ((row >> 5) & 3) * 4;
 }
 
+// Two fp32 operations an instruction.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    uint64_t r, x = *reinterpret_cast<uint64_t*>(&a), y = *reinterpret_cast<uint64_t*>(&b);
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+    return *reinterpret_cast<float2*>(&r);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    uint64_t r, x = *reinterpret_cast<uint64_t*>(&a), y = *reinterpret_cast<uint64_t*>(&b);
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+    return *reinterpret_cast<float2*>(&r);
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    uint64_t r, x = *reinterpret_cast<uint64_t*>(&a), y = *reinterpret_cast<uint64_t*>(&b), z = *reinterpret_cast<uint64_t*>(&c);
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
+    return *reinterpret_cast<float2*>(&r);
+}
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+// Eight columns as four pairs.
+struct F8 {
+    float2 p[4];
+    __device__ __forceinline__ float operator[](int e) const { return (e & 1) ? p[e >> 1].y : p[e >> 1].x; }
+};
+
 // 8 floats -> 8 E2M1 codes (round to nearest even, saturating), v[0] lowest.
-__device__ __forceinline__ uint32_t e2m1_encode8(const float (&v)[8]) {
+__device__ __forceinline__ uint32_t e2m1_encode8(const F8& v) {
     uint32_t r;
     asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
         "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
@@ -57,7 +80,7 @@ __device__ __forceinline__ uint32_t e2m1_encode8(const float (&v)[8]) {
     return r;
 }
 // 8 codes -> 8 floats (exact).
-__device__ __forceinline__ void e2m1_decode8(uint32_t c, float (&v)[8]) {
+__device__ __forceinline__ void e2m1_decode8(uint32_t c, F8& v) {
     uint32_t h[4];
     asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
         "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
@@ -69,9 +92,7 @@ __device__ __forceinline__ void e2m1_decode8(uint32_t c, float (&v)[8]) {
         : "r"(c));
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const float2 f = __half22float2(*reinterpret_cast<__half2*>(&h[i]));
-        v[2 * i] = f.x;
-        v[2 * i + 1] = f.y;
+        v.p[i] = __half22float2(*reinterpret_cast<__half2*>(&h[i]));
     }
 }
 __device__ __forceinline__ float mx4_scale_value(int fmt, uint32_t byte) {
@@ -82,7 +103,7 @@ __device__ __forceinline__ float mx4_scale_value(int fmt, uint32_t byte) {
 
 // Magnitude bits of the largest of 8 values: infinities and NaN order above
 // every finite value, so a block or row that holds one is seen from its maximum.
-__device__ __forceinline__ uint32_t amax_bits8(const float (&v)[8]) {
+__device__ __forceinline__ uint32_t amax_bits8(const F8& v) {
     uint32_t m = 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) m = max(m, __float_as_uint(v[e]) & 0x7FFFFFFFu);
@@ -90,26 +111,41 @@ __device__ __forceinline__ uint32_t amax_bits8(const float (&v)[8]) {
 }
 constexpr uint32_t kInfBits = 0x7F800000u;
 
-// The row's level A of NVFP4 and its stored scale.  Rows below 2688 * 2^-110
-// keep A there, so no reciprocal below overflows; a row with an infinity or
-// NaN has scale NaN (its codes and block scales are zero).
-__device__ __forceinline__ float nv_row_level(uint32_t row_amax_bits) {
-    return fmaxf(__uint_as_float(row_amax_bits), 2688.0f * 0x1p-110f);
+// Row terms of NVFP4 from the row's largest magnitude.
+struct NvRow {
+    float level;    // A
+    float to_s;     // 448 / A
+    float to_code;  // 2688 / A
+    bool ok;        // the row is finite
+};
+// Rows below 2688 * 2^-110 keep A there, so nothing below overflows; a row with
+// an infinity or NaN has scale NaN (its codes and block scales are zero).
+__device__ __forceinline__ NvRow nv_row(uint32_t row_amax_bits) {
+    NvRow r;
+    r.level = fmaxf(__uint_as_float(row_amax_bits), 2688.0f * 0x1p-110f);
+    r.to_s = __fdiv_rn(448.0f, r.level);
+    r.to_code = __fmul_rn(6.0f, r.to_s);
+    r.ok = row_amax_bits < kInfBits;
+    return r;
 }
 __device__ __forceinline__ float nv_row_scale(uint32_t row_amax_bits, float level) {
     if (row_amax_bits == 0u) return 1.0f;
     if (row_amax_bits >= kInfBits) return __uint_as_float(0x7FC00000u);
     return __fdiv_rn(level, 2688.0f);
 }
+__device__ __forceinline__ float rcp_approx(float x) {  // relative error below 2^-22
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
 
 // Codes of this thread's 8 columns and the scale byte of its block.  Every lane
-// of the warp takes part.  level: nv_row_level (NVFP4); ok: the row is finite
-// (NVFP4 only; MXFP4 decides by block).
+// of the warp takes part.  a: magnitude bits of the largest of the 8 (amax_bits8).
 template <int F>
-__device__ __forceinline__ uint32_t mx4_encode(const float (&v)[8], float level, bool ok, uint32_t* byte) {
-    uint32_t a = amax_bits8(v);
+__device__ __forceinline__ uint32_t mx4_encode(const F8& v, uint32_t a, const NvRow& row, uint32_t* byte) {
     a = max(a, __shfl_xor_sync(0xffffffffu, a, 1));
-    float q[8];
+    F8 q;
+    bool ok;
     if (F == kMXFP4) {
         a = max(a, __shfl_xor_sync(0xffffffffu, a, 2));
         const int e = max(static_cast<int>(a >> 23) - 2, 0);
@@ -117,22 +153,24 @@ __device__ __forceinline__ uint32_t mx4_encode(const float (&v)[8], float level,
         *byte = ok ? static_cast<uint32_t>(e) : 0xFFu;
         const float inv = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);  // 2^(127 - e), exact
 #pragma unroll
-        for (int i = 0; i < 8; ++i) q[i] = __fmul_rn(v[i], inv);
+        for (int i = 0; i < 4; ++i) q.p[i] = mul2(v.p[i], both(inv));
     } else {
-        // Both quotients of bf16 values often fall right on a rounding border
-        // (they are ratios of small integers).  The first is a correctly rounded
-        // division of exact operands, so a border stays a border and goes to
-        // even; the second is a product with a rounded reciprocal, brought back
-        // onto the grid of 2^-17 by adding and subtracting 96 (|q| < 9): its
-        // error is below 2^-20 and a bf16 quotient that is no border is at
-        // least 2^-15 away from one.
-        const float lv = level * 0x1p-10f;
-        const float s = __fdiv_rn(__uint_as_float(a) * 0.4375f, lv);
-        *byte = ok ? ocp_encode2<kE4M3>(s, 0.0f) & 0xFFu : 0u;
+        // Quotients of bf16 values often fall right on a rounding border (they are
+        // ratios of small integers), and have to stay there to go to even.  Products
+        // with rounded reciprocals move them by less than 2^-22 of themselves (codes:
+        // 2^-21.4, of at most 5), so they are brought onto a grid first: the
+        // scale's quotient to 20 mantissa bits, the code's to multiples of 2^-17 (96
+        // added and subtracted; |q| < 9).  Quotients of bf16 values that are no border
+        // are at least 2^-13 (relative) and 2^-15 away from one.  With two correctly
+        // rounded divisions a lane instead the quantize was bound by its arithmetic
+        // (8192 x 4096 bf16: 25.1 us).
+        ok = row.ok;
+        const uint32_t s = (__float_as_uint(__fmul_rn(__uint_as_float(a), row.to_s)) + 4u) & ~7u;
+        *byte = ok ? ocp_encode2<kE4M3>(__uint_as_float(s), 0.0f) & 0xFFu : 0u;
         const float sv = ocp_decode2<kE4M3>(*byte).x;
-        const float inv = sv > 0.0f ? __fdiv_rn(2.625f, __fmul_rn(sv, lv)) : 0.0f;
+        const float inv = sv > 0.0f ? __fmul_rn(rcp_approx(sv), row.to_code) : 0.0f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) q[i] = __fsub_rn(__fmaf_rn(v[i], inv, 96.0f), 96.0f);
+        for (int i = 0; i < 4; ++i) q.p[i] = add2(fma2(v.p[i], both(inv), both(96.0f)), both(-96.0f));
     }
     return ok ? e2m1_encode8(q) : 0u;
 }
@@ -175,13 +213,39 @@ struct Raw8 {
     uint4 q[sizeof(In) / 2];
 };
 template <class In>
-__device__ __forceinline__ void unpack8(const Raw8<In>& r, float (&v)[8]) {
+__device__ __forceinline__ F8 unpack8(const Raw8<In>& r) {
+    F8 f;
+    if constexpr (sizeof(In) == 4) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = vec_elem<In>(r.q[sizeof(In) == 4 ? e / 4 : 0], sizeof(In) == 4 ? e % 4 : e);
+        for (int i = 0; i < 2; ++i) {
+            f.p[2 * i] = make_float2(__uint_as_float(r.q[i].x), __uint_as_float(r.q[i].y));
+            f.p[2 * i + 1] = make_float2(__uint_as_float(r.q[i].z), __uint_as_float(r.q[i].w));
+        }
+    } else {
+        const uint32_t w[4] = {r.q[0].x, r.q[0].y, r.q[0].z, r.q[0].w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f.p[i] = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xFFFF0000u));
+    }
+    return f;
+}
+// amax_bits8 of a vector as loaded; bf16 two values an instruction.
+template <class In>
+__device__ __forceinline__ uint32_t amax_bits_raw(const Raw8<In>& r) {
+    if constexpr (sizeof(In) == 2) {
+        const uint4& q = r.q[0];
+        const uint32_t m = __vmaxu2(__vmaxu2(q.x & 0x7FFF7FFFu, q.y & 0x7FFF7FFFu), __vmaxu2(q.z & 0x7FFF7FFFu, q.w & 0x7FFF7FFFu));
+        return max(m & 0xFFFF0000u, m << 16);
+    } else {
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(sizeof(In) / 2); ++i)
+            m = max(max(m, max(r.q[i].x & 0x7FFFFFFFu, r.q[i].y & 0x7FFFFFFFu)), max(r.q[i].z & 0x7FFFFFFFu, r.q[i].w & 0x7FFFFFFFu));
+        return m;
+    }
 }
 // Rounds 8 values to the type (nearest even).
 template <class In>
-__device__ __forceinline__ Raw8<In> pack8(const float (&v)[8]) {
+__device__ __forceinline__ Raw8<In> pack8(const F8& v) {
     Raw8<In> r;
     if constexpr (sizeof(In) == 4) {
 #pragma unroll

@@ -43,18 +43,6 @@ struct MxEpi {
 __device__ __forceinline__ float mx_epi(float acc, float row, float cs, float b) {
     return __fadd_rn(__fmul_rn(__fmul_rn(acc, row), cs), b);
 }
-// Two fp32 operations an instruction.
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-    uint64_t r, x = *reinterpret_cast<uint64_t*>(&a), y = *reinterpret_cast<uint64_t*>(&b);
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
-    return *reinterpret_cast<float2*>(&r);
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-    uint64_t r, x = *reinterpret_cast<uint64_t*>(&a), y = *reinterpret_cast<uint64_t*>(&b);
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
-    return *reinterpret_cast<float2*>(&r);
-}
-
 // Keeps the compiler from using registers that tcgen05.ld fills before the wait
 // that precedes this call.
 template <int NR>

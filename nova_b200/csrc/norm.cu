@@ -35,8 +35,8 @@ struct NormArgs {
     float* scales;       // per row (8-bit, NVFP4)
     int rows, cols;
     size_t x_stride, res_stride;
-    float eps;
-    int w_bf16;
+    float eps, inv_cols;
+    int w_kind;  // bit 0: bf16, bit 1: 16-byte aligned
 };
 
 // The warp's buffer for rows that are not aligned (one kWarpBuf per warp).
@@ -50,21 +50,50 @@ __device__ __forceinline__ uint8_t* warp_buf() {
     }
 }
 
-template <bool VEC>
-__device__ __forceinline__ void load_weight8(const void* w, int w_bf16, int v, int cols, float (&f)[8], uint8_t* buf) {
-    if (w_bf16) unpack8<uint16_t>(load_vec<uint16_t, VEC>(static_cast<const uint16_t*>(w), v, cols, buf), f);
-    else unpack8<float>(load_vec<float, VEC>(static_cast<const float*>(w), v, cols, buf), f);
+// Columns [8v, 8v + 8) of the weight; a vector starts on a 16-byte boundary
+// wherever the weight itself does, whatever the rows do (w_vec).
+template <class W>
+__device__ __forceinline__ F8 load_weight8_of(const W* w, bool w_vec, int v, int cols) {
+    if (w_vec && 8 * v + 8 <= cols) {
+        Raw8<W> r;
+#pragma unroll
+        for (int j = 0; j < static_cast<int>(sizeof(W) / 2); ++j)
+            r.q[j] = __ldg(reinterpret_cast<const uint4*>(w + 8 * static_cast<size_t>(v)) + j);
+        return unpack8<W>(r);
+    }
+    float f[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const int c = 8 * v + e;
+        f[e] = c >= cols ? 0.0f : (sizeof(W) == 4 ? __ldg(reinterpret_cast<const float*>(w) + c)
+                                                  : bf16_bits_to_f32(__ldg(reinterpret_cast<const uint16_t*>(w) + c)));
+    }
+    return F8{{{f[0], f[1]}, {f[2], f[3]}, {f[4], f[5]}, {f[6], f[7]}}};
+}
+__device__ __forceinline__ F8 load_weight8(const void* w, int w_kind, int v, int cols) {
+    return (w_kind & 1) ? load_weight8_of(static_cast<const uint16_t*>(w), w_kind & 2, v, cols)
+                        : load_weight8_of(static_cast<const float*>(w), w_kind & 2, v, cols);
 }
 
 // h = x + residual rounded to the type: the stored value is the one normalized.
 template <class In>
 __device__ __forceinline__ Raw8<In> add8(const Raw8<In>& x, const Raw8<In>& res) {
-    float a[8], b[8];
-    unpack8<In>(x, a);
-    unpack8<In>(res, b);
+    F8 a = unpack8<In>(x);
+    const F8 b = unpack8<In>(res);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) a[e] = __fadd_rn(a[e], b[e]);
+    for (int i = 0; i < 4; ++i) a.p[i] = add2(a.p[i], b.p[i]);
     return pack8<In>(a);
+}
+// t = h w; ss += h^2, tm = max(tm, |t|).
+__device__ __forceinline__ F8 row_terms(const F8& h, const F8& w, float2& ss, uint32_t& tm) {
+    F8 t;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        ss = fma2(h.p[i], h.p[i], ss);
+        t.p[i] = mul2(h.p[i], w.p[i]);
+    }
+    tm = max(tm, amax_bits8(t));
+    return t;
 }
 
 // Sum of `s` and maximum of `m` over the block (every thread gets both).  Two
@@ -90,54 +119,62 @@ __device__ __forceinline__ void block_sum_max(float& s, uint32_t& m, int parity)
 
 // What a row's reduction gives the encoder.
 struct RowNorm {
-    float r;      // 1 / rms
-    float level;  // 8 bits: qmax / T; NVFP4: A
-    bool ok;      // every t of the row is finite
+    float r;        // 1 / rms (where it is needed: y, MXFP4)
+    float to_code;  // 8 bits: qmax / T
+    NvRow nv;       // NVFP4
 };
+__device__ __forceinline__ float row_r(float sumsq, float inv_cols, float eps) {
+    return rsqrtf(__fmaf_rn(sumsq, inv_cols, eps));
+}
+// `first`: this thread stores the row's scale (the only place, besides y and
+// MXFP4, where r and its divisions are needed).
 template <int OUT>
-__device__ __forceinline__ RowNorm row_norm(float sumsq, uint32_t tmax, int cols, float eps, float* scale) {
-    RowNorm n;
-    n.r = __frsqrt_rn(__fadd_rn(__fdiv_rn(sumsq, static_cast<float>(cols)), eps));
-    n.ok = tmax < kInfBits;
-    n.level = 0.0f;
+__device__ __forceinline__ RowNorm row_norm(const NormArgs& a, int row, float sumsq, uint32_t tmax, bool first) {
+    RowNorm n{};
+    if (a.y || OUT == kOutMX) n.r = row_r(sumsq, a.inv_cols, a.eps);
     if (OUT <= kOutINT8) {
         constexpr float qmax = FmtTraits<OUT <= kOutINT8 ? OUT : 0>::qmax;
         const float T = fmaxf(__uint_as_float(tmax), 0x1p-110f);
-        n.level = __fdiv_rn(qmax, T);
-        *scale = !n.ok ? __uint_as_float(0x7FC00000u) : (tmax == 0u ? 1.0f : __fdiv_rn(__fmul_rn(n.r, T), qmax));
+        n.to_code = __fdiv_rn(qmax, T);
+        if (first)
+            a.scales[row] = tmax >= kInfBits ? __uint_as_float(0x7FC00000u)
+                                             : (tmax == 0u ? 1.0f : __fdiv_rn(__fmul_rn(row_r(sumsq, a.inv_cols, a.eps), T), qmax));
     } else if (OUT == kOutNV) {
-        n.level = nv_row_level(tmax);
-        const float g = nv_row_scale(tmax, n.level);
-        *scale = tmax == 0u ? 1.0f : __fmul_rn(n.r, g);
+        n.nv = nv_row(tmax);
+        if (first)
+            a.scales[row] = tmax == 0u ? 1.0f : __fmul_rn(row_r(sumsq, a.inv_cols, a.eps), nv_row_scale(tmax, n.nv.level));
     }
     return n;
 }
 
 // Encodes and stores this thread's 8 columns of a row (every lane takes part).
 template <class In, int OUT, bool VEC>
-__device__ __forceinline__ void emit8(const NormArgs& a, int row, int v, int pitch_words, int words, const float (&t)[8],
+__device__ __forceinline__ void emit8(const NormArgs& a, int row, int v, int pitch_words, int words, const F8& t,
                                       const RowNorm& n, uint8_t* buf) {
     if (a.y || OUT == kOutMX) {
-        float y[8];
+        F8 y;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = __fmul_rn(t[e], n.r);
+        for (int i = 0; i < 4; ++i) y.p[i] = mul2(t.p[i], both(n.r));
         if (a.y) store_vec<In, VEC>(static_cast<In*>(a.y) + static_cast<size_t>(row) * a.cols, v, a.cols, pack8<In>(y), buf);
         if (OUT == kOutMX) {
             uint32_t byte;
-            const uint32_t c = mx4_encode<kMXFP4>(y, 0.0f, true, &byte);
+            const uint32_t c = mx4_encode<kMXFP4>(y, amax_bits8(y), n.nv, &byte);
             mx4_store<kMXFP4>(a.codes + row * mx4_pitch(a.cols), a.bscales, row, v, pitch_words, words, c, byte);
         }
     }
     if (OUT == kOutNV) {
         uint32_t byte;
-        const uint32_t c = mx4_encode<kNVFP4>(t, n.level, n.ok, &byte);
+        const uint32_t c = mx4_encode<kNVFP4>(t, amax_bits8(t), n.nv, &byte);
         mx4_store<kNVFP4>(a.codes + row * mx4_pitch(a.cols), a.bscales, row, v, pitch_words, words, c, byte);
     }
     if (OUT <= kOutINT8) {
         constexpr int F = OUT <= kOutINT8 ? OUT : 0;
         uint32_t c[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) c[i] = ocp_encode2<F>(__fmul_rn(t[2 * i], n.level), __fmul_rn(t[2 * i + 1], n.level));
+        for (int i = 0; i < 4; ++i) {
+            const float2 q = mul2(t.p[i], both(n.to_code));
+            c[i] = ocp_encode2<F>(q.x, q.y);
+        }
         store_codes8<VEC>(a.codes + static_cast<size_t>(row) * a.cols, v, a.cols, make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16)), buf);
     }
 }
@@ -166,31 +203,21 @@ __global__ void __launch_bounds__(256) k_norm_two_pass(const NormArgs a) {
             const Raw8<In> h = load_vec<In, VEC>(x, v, a.cols, buf);
             return res ? add8<In>(h, load_vec<In, VEC>(res, v, a.cols, buf)) : h;
         };
-        float ss = 0.0f;
+        float2 s2 = both(0.0f);
         uint32_t tm = 0;
         for (int v = threadIdx.x; v - lane < nvec; v += blockDim.x) {
             const Raw8<In> hr = load_h(v);
             if (sum) store_vec<In, VEC>(sum, v, a.cols, hr, buf);
-            float h[8], w[8];
-            unpack8<In>(hr, h);
-            load_weight8<VEC>(a.w, a.w_bf16, v, a.cols, w, buf);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                ss = __fmaf_rn(h[e], h[e], ss);
-                w[e] = __fmul_rn(h[e], w[e]);
-            }
-            tm = max(tm, amax_bits8(w));
+            (void)row_terms(unpack8<In>(hr), load_weight8(a.w, a.w_kind, v, a.cols), s2, tm);
         }
+        float ss = s2.x + s2.y;
         block_sum_max(ss, tm, parity);  // (its barrier also orders the unaligned rows' stores before the loads below)
-        float scale = 0.0f;
-        const RowNorm n = row_norm<OUT>(ss, tm, a.cols, a.eps, &scale);
-        if (threadIdx.x == 0 && (OUT <= kOutINT8 || OUT == kOutNV)) a.scales[row] = scale;
+        const RowNorm n = row_norm<OUT>(a, row, ss, tm, threadIdx.x == 0);
         for (int v = threadIdx.x; v - lane < nstep; v += blockDim.x) {
-            float t[8], w[8];
-            unpack8<In>(sum ? load_vec<In, VEC>(sum, v, a.cols, buf) : load_h(v), t);
-            load_weight8<VEC>(a.w, a.w_bf16, v, a.cols, w, buf);
+            F8 t = unpack8<In>(sum ? load_vec<In, VEC>(sum, v, a.cols, buf) : load_h(v));
+            const F8 w = load_weight8(a.w, a.w_kind, v, a.cols);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) t[e] = __fmul_rn(t[e], w[e]);
+            for (int i = 0; i < 4; ++i) t.p[i] = mul2(t.p[i], w.p[i]);
             emit8<In, OUT, VEC>(a, row, v, pitch_words, words, t, n, buf);
         }
     }
@@ -230,20 +257,12 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) k_norm_rows(const NormArgs 
                 for (int i = 0; i < NV; ++i) store_vec<In, VEC>(sum, t0 + i * width, a.cols, h[i], buf);
             }
         }
-        float ss = 0.0f;
+        float2 s2 = both(0.0f);
         uint32_t tm = 0;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            float f[8], w[8];
-            unpack8<In>(h[i], f);
-            load_weight8<VEC>(a.w, a.w_bf16, t0 + i * width, a.cols, w, buf);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                ss = __fmaf_rn(f[e], f[e], ss);
-                w[e] = __fmul_rn(f[e], w[e]);
-            }
-            tm = max(tm, amax_bits8(w));
-        }
+        for (int i = 0; i < NV; ++i)
+            (void)row_terms(unpack8<In>(h[i]), load_weight8(a.w, a.w_kind, t0 + i * width, a.cols), s2, tm);
+        float ss = s2.x + s2.y;
         if (WARP) {
 #pragma unroll
             for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
@@ -251,18 +270,15 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) k_norm_rows(const NormArgs 
         } else {
             block_sum_max(ss, tm, parity);
         }
-        float scale = 0.0f;
-        const RowNorm n = row_norm<OUT>(ss, tm, a.cols, a.eps, &scale);
-        if (t0 == 0 && (OUT <= kOutINT8 || OUT == kOutNV)) a.scales[row] = scale;
+        const RowNorm n = row_norm<OUT>(a, row, ss, tm, t0 == 0);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int v = t0 + i * width;
-            float f[8], w[8];
-            unpack8<In>(h[i], f);
-            load_weight8<VEC>(a.w, a.w_bf16, v, a.cols, w, buf);
+            F8 t = unpack8<In>(h[i]);
+            const F8 w = load_weight8(a.w, a.w_kind, v, a.cols);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) f[e] = __fmul_rn(f[e], w[e]);
-            emit8<In, OUT, VEC>(a, row, v, pitch_words, words, f, n, buf);
+            for (int j = 0; j < 4; ++j) t.p[j] = mul2(t.p[j], w.p[j]);
+            emit8<In, OUT, VEC>(a, row, v, pitch_words, words, t, n, buf);
         }
     }
 }
@@ -276,8 +292,8 @@ struct GradArgs {
     void* dx;          // or NULL
     int rows, cols;
     size_t h_stride;
-    float eps;
-    int w_bf16;
+    float eps, inv_cols;
+    int w_kind;  // bit 0: bf16, bit 1: 16-byte aligned
 };
 
 // Sum of two values over the block.
@@ -304,17 +320,37 @@ __device__ __forceinline__ void block_sum2(float& s, float& g, int parity) {
     }
 }
 
-// Row terms of the gradient: dx = dsum + r (g - h c), c = r mean(g n), n = h r
+// Row terms of the gradient: dx = dsum + r g - c h, c = r^2 mean(g n), n = h r
 // (the bounded form: |mean(g n)| <= max |g|).
 struct RowGrad {
     float r, c;
 };
-__device__ __forceinline__ RowGrad row_grad(float sumsq, float sgh, int cols, float eps) {
-    const float n = static_cast<float>(cols);
+__device__ __forceinline__ RowGrad row_grad(const GradArgs& a, float sumsq, float sgh) {
     RowGrad q;
-    q.r = __frsqrt_rn(__fadd_rn(__fdiv_rn(sumsq, n), eps));
-    q.c = __fmul_rn(__fdiv_rn(__fmul_rn(sgh, q.r), n), q.r);
+    q.r = row_r(sumsq, a.inv_cols, a.eps);
+    q.c = __fmul_rn(__fmul_rn(__fmul_rn(sgh, q.r), a.inv_cols), __fmul_rn(q.r, q.r));
     return q;
+}
+// gw = g w; ss += h^2, sg += gw h.
+__device__ __forceinline__ F8 grad_terms(const F8& h, const F8& g, const F8& w, float2& ss, float2& sg) {
+    F8 gw;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        ss = fma2(h.p[i], h.p[i], ss);
+        gw.p[i] = mul2(g.p[i], w.p[i]);
+        sg = fma2(gw.p[i], h.p[i], sg);
+    }
+    return gw;
+}
+// r gw - c h [+ d]
+__device__ __forceinline__ F8 grad_dx(const F8& h, const F8& gw, const RowGrad& q, bool has_d, const F8& d) {
+    F8 o;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        o.p[i] = has_d ? fma2(both(-q.c), h.p[i], d.p[i]) : mul2(both(-q.c), h.p[i]);
+        o.p[i] = fma2(both(q.r), gw.p[i], o.p[i]);
+    }
+    return o;
 }
 
 // One block per row in two passes, for rows too wide for k_norm_grad; r of every
@@ -332,137 +368,141 @@ __global__ void __launch_bounds__(256) k_norm_grad_rows(const GradArgs a, float*
         const In* hp = static_cast<const In*>(a.h) + row * a.h_stride;
         const size_t at = static_cast<size_t>(row) * a.cols;
         const In* dyp = static_cast<const In*>(a.dy) + at;
-        float ss = 0.0f, sg = 0.0f;
-        for (int v = threadIdx.x; v - lane < nvec; v += blockDim.x) {
-            float h[8], g[8], w[8];
-            unpack8<In>(load_vec<In, VEC>(hp, v, a.cols, buf), h);
-            unpack8<In>(load_vec<In, VEC>(dyp, v, a.cols, buf), g);
-            load_weight8<VEC>(a.w, a.w_bf16, v, a.cols, w, buf);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                ss = __fmaf_rn(h[e], h[e], ss);
-                sg = __fmaf_rn(__fmul_rn(g[e], w[e]), h[e], sg);
-            }
-        }
+        float2 s2 = both(0.0f), g2 = both(0.0f);
+        for (int v = threadIdx.x; v - lane < nvec; v += blockDim.x)
+            (void)grad_terms(unpack8<In>(load_vec<In, VEC>(hp, v, a.cols, buf)), unpack8<In>(load_vec<In, VEC>(dyp, v, a.cols, buf)),
+                             load_weight8(a.w, a.w_kind, v, a.cols), s2, g2);
+        float ss = s2.x + s2.y, sg = g2.x + g2.y;
         block_sum2(ss, sg, parity);
-        const RowGrad q = row_grad(ss, sg, a.cols, a.eps);
+        const RowGrad q = row_grad(a, ss, sg);
         if (threadIdx.x == 0) rs[row] = q.r;
         if (!a.dx) continue;
         for (int v = threadIdx.x; v - lane < nvec; v += blockDim.x) {
-            float h[8], g[8], w[8], d[8];
-            unpack8<In>(load_vec<In, VEC>(hp, v, a.cols, buf), h);
-            unpack8<In>(load_vec<In, VEC>(dyp, v, a.cols, buf), g);
-            load_weight8<VEC>(a.w, a.w_bf16, v, a.cols, w, buf);
-            if (a.dsum) unpack8<In>(load_vec<In, VEC>(static_cast<const In*>(a.dsum) + at, v, a.cols, buf), d);
+            const F8 h = unpack8<In>(load_vec<In, VEC>(hp, v, a.cols, buf));
+            const F8 w = load_weight8(a.w, a.w_kind, v, a.cols);
+            F8 g = unpack8<In>(load_vec<In, VEC>(dyp, v, a.cols, buf)), d{};
+            if (a.dsum) d = unpack8<In>(load_vec<In, VEC>(static_cast<const In*>(a.dsum) + at, v, a.cols, buf));
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                g[e] = __fmul_rn(q.r, __fmaf_rn(-h[e], q.c, __fmul_rn(g[e], w[e])));
-                if (a.dsum) g[e] = __fadd_rn(g[e], d[e]);
-            }
-            store_vec<In, VEC>(static_cast<In*>(a.dx) + at, v, a.cols, pack8<In>(g), buf);
+            for (int i = 0; i < 4; ++i) g.p[i] = mul2(g.p[i], w.p[i]);
+            store_vec<In, VEC>(static_cast<In*>(a.dx) + at, v, a.cols, pack8<In>(grad_dx(h, g, q, a.dsum, d)), buf);
         }
     }
 }
 
-// Rows held in registers, read once: dx, and the weight's gradient summed over
-// the block's rows (blockIdx.x, + gridDim.x, ...) in registers, one partial row a
-// block.  WARP: a warp per row; the block's warps are added in order at the end.
-template <class In, bool VEC, int NV, bool WARP>
-__global__ void __launch_bounds__(WARP ? 256 : 512) k_norm_grad(const GradArgs a, float* __restrict__ part) {
+// A row in registers: its vectors as loaded.
+template <class In, int NV>
+struct GradRow {
+    Raw8<In> h[NV], g[NV], d[NV];
+};
+// The row's sums over the block, its dx, and its share of the weight's gradient.
+// next() runs once every thread of the block has read the row.
+template <class In, bool VEC, int NV, class Next>
+__device__ __forceinline__ void grad_row(const GradArgs& a, const GradRow<In, NV>& r, size_t at, int t0, int width, int parity,
+                                         F8 (&acc)[NV], uint8_t* buf, Next next) {
+    float2 s2 = both(0.0f), g2 = both(0.0f);
+    F8 h[NV], gw[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        h[i] = unpack8<In>(r.h[i]);
+        gw[i] = grad_terms(h[i], unpack8<In>(r.g[i]), load_weight8(a.w, a.w_kind, t0 + i * width, a.cols), s2, g2);
+    }
+    float ss = s2.x + s2.y, sg = g2.x + g2.y;
+    block_sum2(ss, sg, parity);
+    next();
+    const RowGrad q = row_grad(a, ss, sg);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const F8 g = unpack8<In>(r.g[i]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i].p[j] = fma2(mul2(h[i].p[j], both(q.r)), g.p[j], acc[i].p[j]);
+        if (a.dx) {
+            F8 d{};
+            if (a.dsum) d = unpack8<In>(r.d[i]);
+            store_vec<In, VEC>(static_cast<In*>(a.dx) + at, t0 + i * width, a.cols,
+                               pack8<In>(grad_dx(h[i], gw[i], q, a.dsum, d)), buf);
+        }
+    }
+}
+
+// Rows read once: dx, and the weight's gradient summed over the block's rows
+// (blockIdx.x, + gridDim.x, ...) in registers, one partial row a block.
+// Aligned rows (VEC) come through a ring in shared memory by 1-D bulk copies:
+// the next rows stream in while one is reduced, without registers for
+// them (8192 x 4096 bf16: 79 us with loads straight to registers).
+template <class In, bool VEC, int NV>
+__global__ void __launch_bounds__(512) k_norm_grad(const GradArgs a, int stages, float* __restrict__ part, uint32_t* err) {
+    extern __shared__ __align__(128) uint8_t g_smem[];
     pdl_launch_dependents();
     uint8_t* buf = warp_buf<VEC>();
-    const int width = WARP ? 32 : blockDim.x;
-    const int t0 = WARP ? lane_of() : threadIdx.x;
-    const int per = WARP ? blockDim.x >> 5 : 1;
-    pdl_wait();
-    float acc[NV][8];
+    const int t0 = threadIdx.x, width = blockDim.x;
+    const bool has_d = a.dsum && a.dx;
+    F8 acc[NV];
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) acc[i][e] = 0.0f;
+    for (int i = 0; i < NV; ++i) acc[i] = F8{};
     int parity = 0;
-    for (long long rl = static_cast<long long>(blockIdx.x) * per + (WARP ? threadIdx.x >> 5 : 0); rl < a.rows;
-         rl += static_cast<long long>(gridDim.x) * per, parity ^= 1) {
-        const size_t at = static_cast<size_t>(rl) * a.cols;
-        Raw8<In> hr[NV], gr[NV], dr[NV];
-        load_vecs<In, VEC, NV>(hr, static_cast<const In*>(a.h) + static_cast<size_t>(rl) * a.h_stride, t0, width, a.cols, buf);
-        load_vecs<In, VEC, NV>(gr, static_cast<const In*>(a.dy) + at, t0, width, a.cols, buf);
-        if (a.dsum && a.dx) load_vecs<In, VEC, NV>(dr, static_cast<const In*>(a.dsum) + at, t0, width, a.cols, buf);
-        float ss = 0.0f, sg = 0.0f;
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            float h[8], g[8], w[8];
-            unpack8<In>(hr[i], h);
-            unpack8<In>(gr[i], g);
-            load_weight8<VEC>(a.w, a.w_bf16, t0 + i * width, a.cols, w, buf);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                ss = __fmaf_rn(h[e], h[e], ss);
-                sg = __fmaf_rn(__fmul_rn(g[e], w[e]), h[e], sg);
-            }
+    if constexpr (VEC) {
+        const uint32_t rb = static_cast<uint32_t>(a.cols) * sizeof(In);
+        const uint32_t stage_bytes = (has_d ? 3u : 2u) * rb;
+        uint64_t* full = reinterpret_cast<uint64_t*>(g_smem + static_cast<size_t>(stages) * stage_bytes);
+        if (t0 == 0) {
+            for (int k = 0; k < stages; ++k) mbar_init(&full[k], 1);
+            fence_mbar_init();
         }
-        if (WARP) {
-#pragma unroll
-            for (int o = 16; o; o >>= 1) {
-                ss += __shfl_xor_sync(0xffffffffu, ss, o);
-                sg += __shfl_xor_sync(0xffffffffu, sg, o);
+        __syncthreads();
+        pdl_wait();
+        auto issue = [&](long long i) {
+            const long long row = blockIdx.x + i * gridDim.x;
+            if (row >= a.rows) return;
+            const int st = static_cast<int>(i % stages);
+            uint8_t* s = g_smem + static_cast<size_t>(st) * stage_bytes;
+            mbar_arrive_expect_tx(&full[st], stage_bytes);
+            bulk_load_1d(s, static_cast<const In*>(a.h) + static_cast<size_t>(row) * a.h_stride, rb, &full[st]);
+            bulk_load_1d(s + rb, static_cast<const In*>(a.dy) + static_cast<size_t>(row) * a.cols, rb, &full[st]);
+            if (has_d) bulk_load_1d(s + 2 * rb, static_cast<const In*>(a.dsum) + static_cast<size_t>(row) * a.cols, rb, &full[st]);
+        };
+        if (t0 == 0)
+            for (int i = 0; i < stages; ++i) issue(i);
+        int st = 0;
+        uint32_t phase = 0;
+        long long i = 0;
+        bool ok = true;
+        for (; blockIdx.x + i * gridDim.x < a.rows; ++i, parity ^= 1) {
+            const size_t row = static_cast<size_t>(blockIdx.x + i * gridDim.x);
+            ok = mbar_wait(&full[st], phase, err);
+            if (!__syncthreads_and(ok)) {
+                ok = false;
+                break;
             }
-        } else {
-            block_sum2(ss, sg, parity);
+            const uint8_t* s = g_smem + static_cast<size_t>(st) * stage_bytes;
+            GradRow<In, NV> r;
+            load_vecs<In, true, NV>(r.h, reinterpret_cast<const In*>(s), t0, width, a.cols, nullptr);
+            load_vecs<In, true, NV>(r.g, reinterpret_cast<const In*>(s + rb), t0, width, a.cols, nullptr);
+            if (has_d) load_vecs<In, true, NV>(r.d, reinterpret_cast<const In*>(s + 2 * rb), t0, width, a.cols, nullptr);
+            grad_row<In, true, NV>(a, r, row * a.cols, t0, width, parity, acc, nullptr, [&]() {
+                if (t0 == 0) issue(i + stages);
+            });
+            if (++st == stages) { st = 0; phase ^= 1u; }
         }
-        const RowGrad q = row_grad(ss, sg, a.cols, a.eps);
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int v = t0 + i * width;
-            float h[8], g[8];
-            unpack8<In>(hr[i], h);
-            unpack8<In>(gr[i], g);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) acc[i][e] = __fmaf_rn(__fmul_rn(h[e], q.r), g[e], acc[i][e]);
-            if (a.dx) {
-                float w[8], d[8];
-                load_weight8<VEC>(a.w, a.w_bf16, v, a.cols, w, buf);
-                if (a.dsum) unpack8<In>(dr[i], d);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    g[e] = __fmul_rn(q.r, __fmaf_rn(-h[e], q.c, __fmul_rn(g[e], w[e])));
-                    if (a.dsum) g[e] = __fadd_rn(g[e], d[e]);
-                }
-                store_vec<In, VEC>(static_cast<In*>(a.dx) + at, v, a.cols, pack8<In>(g), buf);
+        if (!ok && t0 == 0)  // the copies in flight land before the block ends
+            for (int k = 0; k < stages && blockIdx.x + (i + k) * gridDim.x < a.rows; ++k) {
+                mbar_wait(&full[st], phase, nullptr);
+                if (++st == stages) { st = 0; phase ^= 1u; }
             }
+    } else {
+        pdl_wait();
+        for (long long row = blockIdx.x; row < a.rows; row += gridDim.x, parity ^= 1) {
+            const size_t at = static_cast<size_t>(row) * a.cols;
+            GradRow<In, NV> r;
+            load_vecs<In, VEC, NV>(r.h, static_cast<const In*>(a.h) + static_cast<size_t>(row) * a.h_stride, t0, width, a.cols, buf);
+            load_vecs<In, VEC, NV>(r.g, static_cast<const In*>(a.dy) + at, t0, width, a.cols, buf);
+            if (has_d) load_vecs<In, VEC, NV>(r.d, static_cast<const In*>(a.dsum) + at, t0, width, a.cols, buf);
+            grad_row<In, VEC, NV>(a, r, at, t0, width, parity, acc, buf, []() {});
         }
     }
     if (!part) return;
     float* mine = part + static_cast<size_t>(blockIdx.x) * a.cols;
-    if constexpr (WARP) {
-        __shared__ float s_acc[NV * 256];
-        for (int k = 0; k < per; ++k) {
-            if (static_cast<int>(threadIdx.x >> 5) == k) {
 #pragma unroll
-                for (int i = 0; i < NV; ++i)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        float* s = s_acc + i * 256 + e * 32 + t0;  // column (t0 + 32 i) * 8 + e
-                        *s = k == 0 ? acc[i][e] : __fadd_rn(*s, acc[i][e]);
-                    }
-            }
-            __syncthreads();
-        }
-        for (int c = threadIdx.x; c < a.cols; c += blockDim.x) mine[c] = s_acc[c / 256 * 256 + (c & 7) * 32 + (c / 8 & 31)];
-    } else {
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int c = 8 * (t0 + i * width);
-            if (VEC) {
-                if (c < a.cols) {
-                    reinterpret_cast<float4*>(mine + c)[0] = make_float4(acc[i][0], acc[i][1], acc[i][2], acc[i][3]);
-                    reinterpret_cast<float4*>(mine + c)[1] = make_float4(acc[i][4], acc[i][5], acc[i][6], acc[i][7]);
-                }
-            } else {
-                store_vec<float, VEC>(mine, t0 + i * width, a.cols, pack8<float>(acc[i]), buf);
-            }
-        }
-    }
+    for (int i = 0; i < NV; ++i) store_vec<float, VEC>(mine, t0 + i * width, a.cols, pack8<float>(acc[i]), buf);
 }
 
 // Partial weight gradients: block (x, y) sums dy h r of 256 columns over row
@@ -601,9 +641,9 @@ nq_status_t norm_impl(const char* who, const nq_rmsnorm_desc_t* d, const void* x
     if (st != NQ_SUCCESS) return st;
     const size_t es = d->dtype == NQ_BF16 ? 2 : 4;
     const bool vec = d->cols % 8 == 0 && strided_ok(xs, es) && (!residual || strided_ok(rs, es)) && aligned16(x) &&
-                     aligned16(residual) && aligned16(weight) && aligned16(sum) && aligned16(y) && aligned16(codes);
-    const NormArgs a{x, residual, weight, sum, y, codes, bscales, scales, d->rows, d->cols, xs, rs, d->eps,
-                     d->weight_dtype == NQ_BF16};
+                     aligned16(residual) && aligned16(sum) && aligned16(y) && aligned16(codes);
+    const NormArgs a{x, residual, weight, sum, y, codes, bscales, scales, d->rows, d->cols, xs, rs, d->eps, 1.0f / d->cols,
+                     (d->weight_dtype == NQ_BF16 ? 1 : 0) | (aligned16(weight) ? 2 : 0)};
     const bool bf = d->dtype == NQ_BF16;
     switch (out) {
         case kOutE4M3: return norm_out<kOutE4M3>(a, bf, vec, di, s, who);
@@ -620,21 +660,41 @@ nq_status_t sum_chunks(const float* part, int chunks, int cols, float* dw, cudaS
                        "nq_rmsnorm_backward (weight)");
 }
 
-template <class In, bool VEC, int NV, bool WARP>
-nq_status_t launch_grad(const GradArgs& a, float* dw, int threads, const DeviceInfo& di, cudaStream_t s) {
-    auto kern = k_norm_grad<In, VEC, NV, WARP>;
+constexpr size_t kGradSmem = 200 * 1024;
+
+template <class In, bool VEC, int NV>
+nq_status_t launch_grad(const GradArgs& a, float* dw, const DeviceInfo& di, cudaStream_t s) {
+    auto kern = k_norm_grad<In, VEC, NV>;
+    const int threads = ((a.cols + 8 * NV - 1) / (8 * NV) + 31) / 32 * 32;
+    int stages = 0;
+    size_t smem = 0;
+    if (VEC) {
+        // two to four rows ahead, about 40 KB of them a block
+        const size_t row = static_cast<size_t>(a.cols) * sizeof(In) * (a.dsum && a.dx ? 3 : 2);
+        stages = static_cast<int>(std::max<size_t>(2, std::min<size_t>(4, 60 * 1024 / row)));
+        if (stages * row > kGradSmem) stages = 1;
+        smem = stages * (row + 8);
+        static std::mutex mu;
+        static std::atomic<uint64_t> attr_set{0};
+        nq_status_t st = once_per_device(attr_set, mu, di.device, [&]() -> nq_status_t {
+            NQ_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kGradSmem + 64)),
+                          "cudaFuncSetAttribute(nq_rmsnorm_backward)");
+            return NQ_SUCCESS;
+        });
+        if (st != NQ_SUCCESS) return st;
+    }
     int per_sm = 0;
-    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, threads, 0) != cudaSuccess || per_sm < 1) {
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, threads, smem) != cudaSuccess || per_sm < 1) {
         cudaGetLastError();
         per_sm = 1;
     }
-    const long long blocks = WARP ? (static_cast<long long>(a.rows) + threads / 32 - 1) / (threads / 32) : a.rows;
-    const int grid = static_cast<int>(std::min<long long>(blocks, static_cast<long long>(di.sm_count) * per_sm));
+    const int grid = static_cast<int>(std::min<long long>(a.rows, static_cast<long long>(di.sm_count) * per_sm));
     void* part = nullptr;
     nq_status_t st = NQ_SUCCESS;
     if (dw) st = scratch_alloc(&part, static_cast<size_t>(grid) * a.cols * 4, s);
     if (st != NQ_SUCCESS) return st;
-    st = cuda_status(launch_pdl(kern, dim3(grid), dim3(threads), 0, s, a, static_cast<float*>(part)), "nq_rmsnorm_backward");
+    st = cuda_status(launch_pdl(kern, dim3(grid), dim3(threads), smem, s, a, stages, static_cast<float*>(part), device_error_word()),
+                     "nq_rmsnorm_backward");
     if (st == NQ_SUCCESS && dw) st = sum_chunks(static_cast<const float*>(part), grid, a.cols, dw, s);
     scratch_free(part, s);
     return st;
@@ -642,13 +702,11 @@ nq_status_t launch_grad(const GradArgs& a, float* dw, int threads, const DeviceI
 
 template <class In, bool VEC>
 nq_status_t grad_impl(const GradArgs& a, float* dw, const DeviceInfo& di, cudaStream_t s) {
-    constexpr int NVMAX = sizeof(In) == 2 ? 4 : 2;  // 64 bytes a thread of each tensor
+    // vectors a thread: one up to 64 threads' worth, then two, then (bf16) four
     const int nvec = (a.cols + 7) / 8;
-    if (nvec <= 32) return launch_grad<In, VEC, 1, true>(a, dw, 256, di, s);
-    if (nvec <= 32 * NVMAX) return launch_grad<In, VEC, NVMAX, true>(a, dw, 256, di, s);
-    if (nvec <= 512) return launch_grad<In, VEC, 1, false>(a, dw, (nvec + 31) / 32 * 32, di, s);
-    const int threads = ((nvec + NVMAX - 1) / NVMAX + 31) / 32 * 32;
-    if (threads <= 512) return launch_grad<In, VEC, NVMAX, false>(a, dw, threads, di, s);
+    if (nvec <= 64) return launch_grad<In, VEC, 1>(a, dw, di, s);
+    if (nvec <= 1024) return launch_grad<In, VEC, 2>(a, dw, di, s);
+    if (sizeof(In) == 2 && nvec <= 2048) return launch_grad<In, VEC, sizeof(In) == 2 ? 4 : 2>(a, dw, di, s);
     const int chunks = static_cast<int>(std::min<long long>(64, a.rows));
     const int per = (a.rows + chunks - 1) / chunks;
     void* scratch = nullptr;
@@ -711,10 +769,10 @@ nq_status_t nq_rmsnorm_backward(const nq_rmsnorm_desc_t* desc, const void* h, co
     st = nq::current_device(&di);
     if (st != NQ_SUCCESS) return st;
     const bool bf = desc->dtype == NQ_BF16;
-    const bool vec = desc->cols % 8 == 0 && nq::strided_ok(xs, bf ? 2 : 4) && nq::aligned16(h) && nq::aligned16(weight) &&
+    const bool vec = desc->cols % 8 == 0 && nq::strided_ok(xs, bf ? 2 : 4) && nq::aligned16(h) &&
                      nq::aligned16(grad_y) && nq::aligned16(grad_sum) && nq::aligned16(grad_x);
-    const nq::GradArgs a{h, weight, grad_y, grad_sum, grad_x, desc->rows, desc->cols, xs, desc->eps,
-                         desc->weight_dtype == NQ_BF16};
+    const nq::GradArgs a{h, weight, grad_y, grad_sum, grad_x, desc->rows, desc->cols, xs, desc->eps, 1.0f / desc->cols,
+                         (desc->weight_dtype == NQ_BF16 ? 1 : 0) | (nq::aligned16(weight) ? 2 : 0)};
     if (bf) return vec ? nq::grad_impl<uint16_t, true>(a, grad_weight, di, s) : nq::grad_impl<uint16_t, false>(a, grad_weight, di, s);
     return vec ? nq::grad_impl<float, true>(a, grad_weight, di, s) : nq::grad_impl<float, false>(a, grad_weight, di, s);
 }
