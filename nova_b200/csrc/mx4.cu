@@ -42,13 +42,13 @@ __global__ void __launch_bounds__(kThreads) k_mx4_quant_wide(const In* __restric
     uint8_t* buf = warp_buf<VEC>();
     const int nvec = (cols + 7) / 8;
     const int words = mx4_words(cols, Mx4Traits<F>::block);
-    const int pitch_words = static_cast<int>(mx4_pitch(cols) / 4);
     const int nstep = words * Mx4Traits<F>::word_lanes;
     const int lane = lane_of();
     int parity = 0;
     for (long long rl = blockIdx.x; rl < rows; rl += gridDim.x, parity ^= 1) {
         const int row = static_cast<int>(rl);
         const In* x = src + row * ld;
+        const Mx4Row to = mx4_row(codes, bscales, row, cols, words);
         NvRow nr{};
         if (F == kNVFP4) {
             uint32_t m = 0;
@@ -62,7 +62,7 @@ __global__ void __launch_bounds__(kThreads) k_mx4_quant_wide(const In* __restric
             const Raw8<In> r = load_vec<In, VEC>(x, v, cols, buf);
             uint32_t byte;
             const uint32_t c = mx4_encode<F>(unpack8<In>(r), amax_bits_raw<In>(r), nr, &byte);
-            mx4_store<F>(codes + row * mx4_pitch(cols), bscales, row, v, pitch_words, words, c, byte);
+            mx4_store<F>(to, v, c, byte);
         }
     }
 }
@@ -76,7 +76,6 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) k_mx4_quant(const In* __res
     pdl_launch_dependents();
     uint8_t* buf = warp_buf<VEC>();
     const int words = mx4_words(cols, Mx4Traits<F>::block);
-    const int pitch_words = static_cast<int>(mx4_pitch(cols) / 4);
     const int width = WARP ? 32 : blockDim.x;
     const int t0 = WARP ? lane_of() : threadIdx.x;
     const int per = WARP ? blockDim.x >> 5 : 1;
@@ -87,6 +86,7 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) k_mx4_quant(const In* __res
         const int row = static_cast<int>(rl);
         Raw8<In> x[NV];
         load_vecs<In, VEC, NV>(x, src + row * ld, t0, width, cols, buf);
+        const Mx4Row to = mx4_row(codes, bscales, row, cols, words);
         uint32_t am[NV];
 #pragma unroll
         for (int i = 0; i < NV; ++i) am[i] = amax_bits_raw<In>(x[i]);
@@ -103,7 +103,7 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) k_mx4_quant(const In* __res
         for (int i = 0; i < NV; ++i) {
             uint32_t byte;
             const uint32_t c = mx4_encode<F>(unpack8<In>(x[i]), am[i], nr, &byte);
-            mx4_store<F>(codes + row * mx4_pitch(cols), bscales, row, t0 + i * width, pitch_words, words, c, byte);
+            mx4_store<F>(to, t0 + i * width, c, byte);
         }
     }
 }
@@ -126,6 +126,7 @@ __global__ void __launch_bounds__(kThreads) k_mx4_dequant(const uint8_t* __restr
         const int row = static_cast<int>(rl);
         const float g = rscales ? __ldg(rscales + row) : 1.0f;
         const uint32_t* code = reinterpret_cast<const uint32_t*>(codes + row * mx4_pitch(cols));
+        const uint8_t* scale = bscales + mx4_scale_offset(row, 0, words);
         T* out = dst + static_cast<size_t>(row) * cols;
         for (int v0 = t0; v0 - lane_of() < nvec; v0 += 4 * width) {
             uint32_t c[4], s[4];
@@ -133,7 +134,7 @@ __global__ void __launch_bounds__(kThreads) k_mx4_dequant(const uint8_t* __restr
             for (int i = 0; i < 4; ++i) {
                 const int v = v0 + i * width, b = v / L;
                 c[i] = v < nvec ? __ldg(code + v) : 0u;
-                s[i] = v < nvec ? __ldg(bscales + mx4_scale_offset(row, b / 4, words) + b % 4) : 0u;
+                s[i] = v < nvec ? __ldg(scale + static_cast<size_t>(b / 4) * 512 + b % 4) : 0u;
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {

@@ -103,11 +103,15 @@ __device__ __forceinline__ float mx4_scale_value(int fmt, uint32_t byte) {
 
 // Magnitude bits of the largest of 8 values: infinities and NaN order above
 // every finite value, so a block or row that holds one is seen from its maximum.
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {  // NaN if any of them is
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 __device__ __forceinline__ uint32_t amax_bits8(const F8& v) {
-    uint32_t m = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) m = max(m, __float_as_uint(v[e]) & 0x7FFFFFFFu);
-    return m;
+    const float a = max3_nan(fabsf(v[0]), fabsf(v[1]), fabsf(v[2]));
+    const float b = max3_nan(fabsf(v[3]), fabsf(v[4]), fabsf(v[5]));
+    return __float_as_uint(max3_nan(max3_nan(fabsf(v[6]), fabsf(v[7]), a), b, b)) & 0x7FFFFFFFu;
 }
 constexpr uint32_t kInfBits = 0x7F800000u;
 
@@ -185,15 +189,24 @@ __device__ __forceinline__ uint32_t mx4_scale_word(uint32_t byte) {
     return w;
 }
 
-// Stores one warp step of a quantised row: 8 columns a lane from column 8 * v.
+// Where a quantised row goes.
+struct Mx4Row {
+    uint32_t* codes;
+    uint8_t* scales;  // its word 0; word w is 512 w bytes on
+    int pitch_words, words;
+};
+__device__ __forceinline__ Mx4Row mx4_row(uint8_t* codes, uint8_t* scales, int row, int cols, int words) {
+    const size_t pitch = mx4_pitch(cols);
+    return Mx4Row{reinterpret_cast<uint32_t*>(codes + row * pitch), scales + mx4_scale_offset(row, 0, words),
+                  static_cast<int>(pitch / 4), words};
+}
+// Stores one warp step of it: 8 columns a lane from column 8 * v.
 template <int F>
-__device__ __forceinline__ void mx4_store(uint8_t* codes_row, uint8_t* scales, int row, int v, int pitch_words, int words,
-                                          uint32_t code, uint32_t byte) {
+__device__ __forceinline__ void mx4_store(const Mx4Row& r, int v, uint32_t code, uint32_t byte) {
     const uint32_t w = mx4_scale_word<F>(byte);
     constexpr int WL = Mx4Traits<F>::word_lanes;
-    if (v < pitch_words) reinterpret_cast<uint32_t*>(codes_row)[v] = code;
-    if (v % WL == 0 && v / WL < words)
-        *reinterpret_cast<uint32_t*>(scales + mx4_scale_offset(row, v / WL, words)) = w;
+    if (v < r.pitch_words) r.codes[v] = code;
+    if (v % WL == 0 && v / WL < r.words) *reinterpret_cast<uint32_t*>(r.scales + static_cast<size_t>(v / WL) * 512) = w;
 }
 
 // ---- rows of fp32 / bf16 in vectors of 8 columns -----------------------------------
@@ -236,11 +249,7 @@ __device__ __forceinline__ uint32_t amax_bits_raw(const Raw8<In>& r) {
         const uint32_t m = __vmaxu2(__vmaxu2(q.x & 0x7FFF7FFFu, q.y & 0x7FFF7FFFu), __vmaxu2(q.z & 0x7FFF7FFFu, q.w & 0x7FFF7FFFu));
         return max(m & 0xFFFF0000u, m << 16);
     } else {
-        uint32_t m = 0;
-#pragma unroll
-        for (int i = 0; i < static_cast<int>(sizeof(In) / 2); ++i)
-            m = max(max(m, max(r.q[i].x & 0x7FFFFFFFu, r.q[i].y & 0x7FFFFFFFu)), max(r.q[i].z & 0x7FFFFFFFu, r.q[i].w & 0x7FFFFFFFu));
-        return m;
+        return amax_bits8(unpack8<In>(r));
     }
 }
 // Rounds 8 values to the type (nearest even).

@@ -149,8 +149,7 @@ __device__ __forceinline__ RowNorm row_norm(const NormArgs& a, int row, float su
 
 // Encodes and stores this thread's 8 columns of a row (every lane takes part).
 template <class In, int OUT, bool VEC>
-__device__ __forceinline__ void emit8(const NormArgs& a, int row, int v, int pitch_words, int words, const F8& t,
-                                      const RowNorm& n, uint8_t* buf) {
+__device__ __forceinline__ void emit8(const NormArgs& a, int row, int v, const Mx4Row& to, const F8& t, const RowNorm& n, uint8_t* buf) {
     if (a.y || OUT == kOutMX) {
         F8 y;
 #pragma unroll
@@ -159,13 +158,13 @@ __device__ __forceinline__ void emit8(const NormArgs& a, int row, int v, int pit
         if (OUT == kOutMX) {
             uint32_t byte;
             const uint32_t c = mx4_encode<kMXFP4>(y, amax_bits8(y), n.nv, &byte);
-            mx4_store<kMXFP4>(a.codes + row * mx4_pitch(a.cols), a.bscales, row, v, pitch_words, words, c, byte);
+            mx4_store<kMXFP4>(to, v, c, byte);
         }
     }
     if (OUT == kOutNV) {
         uint32_t byte;
         const uint32_t c = mx4_encode<kNVFP4>(t, amax_bits8(t), n.nv, &byte);
-        mx4_store<kNVFP4>(a.codes + row * mx4_pitch(a.cols), a.bscales, row, v, pitch_words, words, c, byte);
+        mx4_store<kNVFP4>(to, v, c, byte);
     }
     if (OUT <= kOutINT8) {
         constexpr int F = OUT <= kOutINT8 ? OUT : 0;
@@ -190,7 +189,6 @@ __global__ void __launch_bounds__(256) k_norm_two_pass(const NormArgs a) {
     const int nvec = (a.cols + 7) / 8;
     const bool four = OUT == kOutMX || OUT == kOutNV;
     const int words = four ? mx4_words(a.cols, Mx4Traits<F>::block) : 0;
-    const int pitch_words = static_cast<int>(mx4_pitch(a.cols) / 4);
     const int nstep = four ? words * Mx4Traits<F>::word_lanes : nvec;
     const int lane = lane_of();
     int parity = 0;
@@ -212,13 +210,14 @@ __global__ void __launch_bounds__(256) k_norm_two_pass(const NormArgs a) {
         }
         float ss = s2.x + s2.y;
         block_sum_max(ss, tm, parity);  // (its barrier also orders the unaligned rows' stores before the loads below)
+        const Mx4Row to = four ? mx4_row(a.codes, a.bscales, row, a.cols, words) : Mx4Row{};
         const RowNorm n = row_norm<OUT>(a, row, ss, tm, threadIdx.x == 0);
         for (int v = threadIdx.x; v - lane < nstep; v += blockDim.x) {
             F8 t = unpack8<In>(sum ? load_vec<In, VEC>(sum, v, a.cols, buf) : load_h(v));
             const F8 w = load_weight8(a.w, a.w_kind, v, a.cols);
 #pragma unroll
             for (int i = 0; i < 4; ++i) t.p[i] = mul2(t.p[i], w.p[i]);
-            emit8<In, OUT, VEC>(a, row, v, pitch_words, words, t, n, buf);
+            emit8<In, OUT, VEC>(a, row, v, to, t, n, buf);
         }
     }
 }
@@ -233,7 +232,6 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) k_norm_rows(const NormArgs 
     constexpr int F = OUT == kOutNV ? kNVFP4 : kMXFP4;
     const bool four = OUT == kOutMX || OUT == kOutNV;
     const int words = four ? mx4_words(a.cols, Mx4Traits<F>::block) : 0;
-    const int pitch_words = static_cast<int>(mx4_pitch(a.cols) / 4);
     const int width = WARP ? 32 : blockDim.x;
     const int t0 = WARP ? threadIdx.x & 31 : threadIdx.x;
     const int per = WARP ? blockDim.x >> 5 : 1;  // rows a block takes at once
@@ -270,6 +268,7 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) k_norm_rows(const NormArgs 
         } else {
             block_sum_max(ss, tm, parity);
         }
+        const Mx4Row to = four ? mx4_row(a.codes, a.bscales, row, a.cols, words) : Mx4Row{};
         const RowNorm n = row_norm<OUT>(a, row, ss, tm, t0 == 0);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
@@ -278,7 +277,7 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) k_norm_rows(const NormArgs 
             const F8 w = load_weight8(a.w, a.w_kind, v, a.cols);
 #pragma unroll
             for (int j = 0; j < 4; ++j) t.p[j] = mul2(t.p[j], w.p[j]);
-            emit8<In, OUT, VEC>(a, row, v, pitch_words, words, t, n, buf);
+            emit8<In, OUT, VEC>(a, row, v, to, t, n, buf);
         }
     }
 }
