@@ -282,6 +282,75 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) k_norm_rows(const NormArgs 
     }
 }
 
+// Many aligned rows: they come through a ring in shared memory by 1-D bulk
+// copies, so that the next rows stream in while one is reduced and encoded.
+template <class In, int OUT, int NV>
+__global__ void __launch_bounds__(512) k_norm_ring(const NormArgs a, int stages, uint32_t* err) {
+    extern __shared__ __align__(128) uint8_t n_smem[];
+    pdl_launch_dependents();
+    constexpr int F = OUT == kOutNV ? kNVFP4 : kMXFP4;
+    const bool four = OUT == kOutMX || OUT == kOutNV;
+    const int words = four ? mx4_words(a.cols, Mx4Traits<F>::block) : 0;
+    const int width = blockDim.x, t0 = threadIdx.x;
+    const uint32_t rb = static_cast<uint32_t>(a.cols) * sizeof(In);
+    const uint32_t stage_bytes = (a.res ? 2u : 1u) * rb;
+    uint64_t* full = reinterpret_cast<uint64_t*>(n_smem + static_cast<size_t>(stages) * stage_bytes);
+    if (t0 == 0) {
+        for (int k = 0; k < stages; ++k) mbar_init(&full[k], 1);
+        fence_mbar_init();
+    }
+    __syncthreads();
+    pdl_wait();
+    long long last = -1;  // the last row issued
+    auto issue = [&](long long i) {
+        const long long row = blockIdx.x + i * gridDim.x;
+        if (row >= a.rows) return;
+        const int st = static_cast<int>(i % stages);
+        uint8_t* s = n_smem + static_cast<size_t>(st) * stage_bytes;
+        last = i;
+        mbar_arrive_expect_tx(&full[st], stage_bytes);
+        bulk_load_1d(s, static_cast<const In*>(a.x) + static_cast<size_t>(row) * a.x_stride, rb, &full[st]);
+        if (a.res) bulk_load_1d(s + rb, static_cast<const In*>(a.res) + static_cast<size_t>(row) * a.res_stride, rb, &full[st]);
+    };
+    if (t0 == 0)
+        for (int i = 0; i < stages; ++i) issue(i);
+    int st = 0, parity = 0;
+    uint32_t phase = 0;
+    bool ok = true;  // after a wait that ran out (error bit set) a thread waits and issues no more
+    for (long long i = 0; blockIdx.x + i * gridDim.x < a.rows; ++i, parity ^= 1) {
+        const int row = static_cast<int>(blockIdx.x + i * gridDim.x);
+        ok = ok && mbar_wait(&full[st], phase, err);
+        const In* s = reinterpret_cast<const In*>(n_smem + static_cast<size_t>(st) * stage_bytes);
+        Raw8<In> h[NV];
+        load_vecs<In, true, NV>(h, s, t0, width, a.cols, nullptr);
+        if (a.res) {
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                const int v = t0 + k * width;
+                h[k] = add8<In>(h[k], load_vec<In, true>(s + a.cols, v, a.cols, nullptr));
+                if (a.sum) store_vec<In, true>(static_cast<In*>(a.sum) + static_cast<size_t>(row) * a.cols, v, a.cols, h[k], nullptr);
+            }
+        }
+        float2 s2 = both(0.0f);
+        uint32_t tm = 0;
+        F8 t[NV];
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+            t[k] = row_terms(unpack8<In>(h[k]), load_weight8(a.w, a.w_kind, t0 + k * width, a.cols), s2, tm);
+        float ss = s2.x + s2.y;
+        block_sum_max(ss, tm, parity);
+        if (t0 == 0 && ok) issue(i + stages);  // every thread has read the stage
+        const Mx4Row to = four ? mx4_row(a.codes, a.bscales, row, a.cols, words) : Mx4Row{};
+        const RowNorm n = row_norm<OUT>(a, row, ss, tm, t0 == 0);
+#pragma unroll
+        for (int k = 0; k < NV; ++k) emit8<In, OUT, true>(a, row, t0 + k * width, to, t[k], n, nullptr);
+        if (++st == stages) { st = 0; phase ^= 1u; }
+    }
+    if (!ok && t0 == 0)  // copies still in flight land before the block ends
+        for (long long k = max(0ll, last - stages + 1); k <= last; ++k)
+            mbar_wait(&full[k % stages], static_cast<uint32_t>(k / stages) & 1u, nullptr);
+}
+
 // ---- gradient ---------------------------------------------------------------------
 struct GradArgs {
     const void* h;
@@ -585,6 +654,32 @@ nq_status_t launch_norm_rows(const NormArgs& a, int threads, const DeviceInfo& d
     return cuda_status(launch_pdl(kern, dim3(grid), dim3(threads), 0, s, a), who);
 }
 
+constexpr size_t kRingSmem = 200 * 1024;
+
+template <class In, int OUT, int NV>
+nq_status_t launch_norm_ring(const NormArgs& a, int nvec, const DeviceInfo& di, cudaStream_t s, const char* who) {
+    auto kern = k_norm_ring<In, OUT, NV>;
+    const int threads = ((nvec + NV - 1) / NV + 31) / 32 * 32;
+    const size_t row = static_cast<size_t>(a.cols) * sizeof(In) * (a.res ? 2 : 1);
+    const int stages = static_cast<int>(std::max<size_t>(2, std::min<size_t>(4, 96 * 1024 / row)));
+    const size_t smem = stages * (row + 8);
+    static std::mutex mu;
+    static std::atomic<uint64_t> attr_set{0};
+    nq_status_t st = once_per_device(attr_set, mu, di.device, [&]() -> nq_status_t {
+        NQ_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kRingSmem)),
+                      "cudaFuncSetAttribute(nq_rmsnorm)");
+        return NQ_SUCCESS;
+    });
+    if (st != NQ_SUCCESS) return st;
+    int per_sm = 0;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, threads, smem) != cudaSuccess || per_sm < 1) {
+        cudaGetLastError();
+        per_sm = 1;
+    }
+    const int grid = static_cast<int>(std::min<long long>(a.rows, static_cast<long long>(di.sm_count) * per_sm));
+    return cuda_status(launch_pdl(kern, dim3(grid), dim3(threads), smem, s, a, stages, device_error_word()), who);
+}
+
 template <class In, int OUT, bool VEC>
 nq_status_t launch_norm(const NormArgs& a, const DeviceInfo& di, cudaStream_t s, const char* who) {
     constexpr int NVMAX = sizeof(In) == 2 ? 4 : 2;  // 64 bytes a thread of each tensor
@@ -598,6 +693,10 @@ nq_status_t launch_norm(const NormArgs& a, const DeviceInfo& di, cudaStream_t s,
     if (a.rows < 2 * di.sm_count && nvec <= 1024)
         return launch_norm_rows<In, OUT, VEC, 1, false>(a, (nvec + 31) / 32 * 32, di, s, who);
     const int threads = ((nvec + NVMAX - 1) / NVMAX + 31) / 32 * 32;
+    if (VEC && a.rows >= 4 * di.sm_count && nvec <= 1024) {
+        if (nvec <= 512) return launch_norm_ring<In, OUT, NVMAX / 2>(a, nvec, di, s, who);
+        return launch_norm_ring<In, OUT, NVMAX>(a, nvec, di, s, who);
+    }
     if (threads <= 1024) return launch_norm_rows<In, OUT, VEC, NVMAX, false>(a, threads, di, s, who);
     const int grid = static_cast<int>(std::min<long long>(a.rows, static_cast<long long>(di.sm_count) * 8));
     return cuda_status(launch_pdl(k_norm_two_pass<In, OUT, VEC>, dim3(grid), dim3(256), 0, s, a), who);
