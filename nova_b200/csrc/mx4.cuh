@@ -143,40 +143,80 @@ __device__ __forceinline__ float rcp_approx(float x) {  // relative error below 
     return r;
 }
 
+// Scale byte of a block from the magnitude bits of its largest value, and the
+// factor that takes its values to E2M1's range.
+struct Mx4Block {
+    uint32_t byte;
+    float inv;
+    double unit;  // NVFP4, FIX: s A
+    bool ok;      // codes are not forced to zero
+};
+// A rounded quotient on a grid (below) stands on a rounding border: `exact` is the sign of the
+// true quotient's distance from it, and a step that no rounding to a few bits sees.
+__device__ __forceinline__ float nudge(float q, double exact) {
+    return exact > 0.0 ? q * (1.0f + 0x1p-20f) : (exact < 0.0 ? q * (1.0f - 0x1p-20f) : q);
+}
+// NVFP4's quotients.  Those of bf16 values often fall right on a rounding border
+// (they are ratios of small integers), and have to stay there to go to even.
+// Products with rounded reciprocals move them by less than 2^-22 of themselves (codes:
+// 2^-21.4, of at most 5), so they are brought onto a grid first: the scale's quotient
+// to 20 mantissa bits, the code's to multiples of 2^-17 (96 added and
+// subtracted; |q| < 9).  Quotients of bf16 values that are no border are at least 2^-13
+// (relative) and 2^-15 away from one, so they round as the true quotient does.
+// FIX, for values of more bits: a quotient that the grid puts on a border (about
+// one in 10^5) is compared with it exactly, in products of double.  With two correctly
+// rounded divisions a lane instead the quantize was bound by its arithmetic (8192 x
+// 4096 bf16: 25.1 us).
+template <int F, bool FIX>
+__device__ __forceinline__ Mx4Block mx4_block(uint32_t a, const NvRow& row) {
+    Mx4Block k;
+    k.unit = 0.0;
+    if (F == kMXFP4) {
+        const int e = max(static_cast<int>(a >> 23) - 2, 0);
+        k.ok = a < kInfBits;
+        k.byte = k.ok ? static_cast<uint32_t>(e) : 0xFFu;
+        k.inv = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);  // 2^(127 - e), exact
+    } else {
+        k.ok = row.ok;
+        const uint32_t g = (__float_as_uint(__fmul_rn(__uint_as_float(a), row.to_s)) + 4u) & ~7u;
+        float s = __uint_as_float(g);
+        if (FIX && (g & 0x7FFFFu) == 0u && g != 0u)  // borders of E4M3 have four mantissa bits
+            s = nudge(s, 448.0 * __uint_as_float(a) - static_cast<double>(s) * row.level);
+        k.byte = k.ok ? ocp_encode2<kE4M3>(s, 0.0f) & 0xFFu : 0u;
+        const float sv = ocp_decode2<kE4M3>(k.byte).x;
+        k.inv = sv > 0.0f ? __fmul_rn(rcp_approx(sv), row.to_code) : 0.0f;
+        if (FIX) k.unit = static_cast<double>(sv) * row.level;
+    }
+    return k;
+}
+template <int F, bool FIX>
+__device__ __forceinline__ uint32_t mx4_codes8(const F8& v, const Mx4Block& k) {
+    F8 q;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        q.p[i] = F == kMXFP4 ? mul2(v.p[i], both(k.inv)) : add2(fma2(v.p[i], both(k.inv), both(96.0f)), both(-96.0f));
+    if (F == kNVFP4 && FIX) {
+        // borders of E2M1 are multiples of 1/4 (adding 1.5 * 2^21 rounds to them)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 r = add2(add2(q.p[i], both(3145728.0f)), both(-3145728.0f));
+            if (r.x == q.p[i].x && r.x != 0.0f)
+                q.p[i].x = nudge(r.x, 2688.0 * fabsf(v.p[i].x) - static_cast<double>(fabsf(r.x)) * k.unit);
+            if (r.y == q.p[i].y && r.y != 0.0f)
+                q.p[i].y = nudge(r.y, 2688.0 * fabsf(v.p[i].y) - static_cast<double>(fabsf(r.y)) * k.unit);
+        }
+    }
+    return k.ok ? e2m1_encode8(q) : 0u;
+}
 // Codes of this thread's 8 columns and the scale byte of its block.  Every lane
 // of the warp takes part.  a: magnitude bits of the largest of the 8 (amax_bits8).
-template <int F>
+template <int F, bool FIX>
 __device__ __forceinline__ uint32_t mx4_encode(const F8& v, uint32_t a, const NvRow& row, uint32_t* byte) {
     a = max(a, __shfl_xor_sync(0xffffffffu, a, 1));
-    F8 q;
-    bool ok;
-    if (F == kMXFP4) {
-        a = max(a, __shfl_xor_sync(0xffffffffu, a, 2));
-        const int e = max(static_cast<int>(a >> 23) - 2, 0);
-        ok = a < kInfBits;
-        *byte = ok ? static_cast<uint32_t>(e) : 0xFFu;
-        const float inv = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);  // 2^(127 - e), exact
-#pragma unroll
-        for (int i = 0; i < 4; ++i) q.p[i] = mul2(v.p[i], both(inv));
-    } else {
-        // Quotients of bf16 values often fall right on a rounding border (they are
-        // ratios of small integers), and have to stay there to go to even.  Products
-        // with rounded reciprocals move them by less than 2^-22 of themselves (codes:
-        // 2^-21.4, of at most 5), so they are brought onto a grid first: the
-        // scale's quotient to 20 mantissa bits, the code's to multiples of 2^-17 (96
-        // added and subtracted; |q| < 9).  Quotients of bf16 values that are no border
-        // are at least 2^-13 (relative) and 2^-15 away from one.  With two correctly
-        // rounded divisions a lane instead the quantize was bound by its arithmetic
-        // (8192 x 4096 bf16: 25.1 us).
-        ok = row.ok;
-        const uint32_t s = (__float_as_uint(__fmul_rn(__uint_as_float(a), row.to_s)) + 4u) & ~7u;
-        *byte = ok ? ocp_encode2<kE4M3>(__uint_as_float(s), 0.0f) & 0xFFu : 0u;
-        const float sv = ocp_decode2<kE4M3>(*byte).x;
-        const float inv = sv > 0.0f ? __fmul_rn(rcp_approx(sv), row.to_code) : 0.0f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) q.p[i] = add2(fma2(v.p[i], both(inv), both(96.0f)), both(-96.0f));
-    }
-    return ok ? e2m1_encode8(q) : 0u;
+    if (F == kMXFP4) a = max(a, __shfl_xor_sync(0xffffffffu, a, 2));
+    const Mx4Block k = mx4_block<F, FIX>(a, row);
+    *byte = k.byte;
+    return mx4_codes8<F, FIX>(v, k);
 }
 
 // The word of four scale bytes of this lane's group of word_lanes lanes (every
@@ -339,6 +379,41 @@ __device__ __forceinline__ void store_codes8(uint8_t* row, int v, int cols, cons
         for (int e = 0; e < 8; ++e)
             if (c0 + 32 * e < cols) row[c0 + 32 * e] = buf[32 * e + lane_of()];
     }
+}
+
+// ---- 16 columns a lane (rows on 32-byte boundaries, cols a multiple of 16) ---------------
+// A lane holds an NVFP4 block or half an MXFP4 block: half the exchanges between
+// lanes and half the work per scale of the 8-column form, and 32-byte accesses.
+struct Word32 {
+    uint32_t w[8];
+};
+__device__ __forceinline__ Word32 ld_global_32(const void* p) {
+    Word32 r;
+    asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r.w[0]), "=r"(r.w[1]), "=r"(r.w[2]), "=r"(r.w[3]), "=r"(r.w[4]), "=r"(r.w[5]), "=r"(r.w[6]), "=r"(r.w[7])
+                 : "l"(p));
+    return r;
+}
+__device__ __forceinline__ void st_global_32(void* p, const Word32& r) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(r.w[0]), "r"(r.w[1]), "r"(r.w[2]),
+                 "r"(r.w[3]), "r"(r.w[4]), "r"(r.w[5]), "r"(r.w[6]), "r"(r.w[7])
+                 : "memory");
+}
+template <class In>
+struct Raw16 {
+    Word32 q[sizeof(In) / 2];
+};
+// Half `i` (0, 1) as a vector of 8 columns.
+template <class In>
+__device__ __forceinline__ Raw8<In> half_of(const Raw16<In>& r, int i) {
+    Raw8<In> h;
+    if constexpr (sizeof(In) == 2) {
+        h.q[0] = make_uint4(r.q[0].w[4 * i], r.q[0].w[4 * i + 1], r.q[0].w[4 * i + 2], r.q[0].w[4 * i + 3]);
+    } else {
+        h.q[0] = make_uint4(r.q[i].w[0], r.q[i].w[1], r.q[i].w[2], r.q[i].w[3]);
+        h.q[1] = make_uint4(r.q[i].w[4], r.q[i].w[5], r.q[i].w[6], r.q[i].w[7]);
+    }
+    return h;
 }
 
 }  // namespace dev

@@ -37,6 +37,7 @@ struct NormArgs {
     size_t x_stride, res_stride;
     float eps, inv_cols;
     int w_kind;  // bit 0: bf16, bit 1: 16-byte aligned
+    int shift0;  // columns from a boundary of 8 to row 0 where all tensors agree on it, else -1 (k_norm_cut)
 };
 
 // The warp's buffer for rows that are not aligned (one kWarpBuf per warp).
@@ -157,13 +158,13 @@ __device__ __forceinline__ void emit8(const NormArgs& a, int row, int v, const M
         if (a.y) store_vec<In, VEC>(static_cast<In*>(a.y) + static_cast<size_t>(row) * a.cols, v, a.cols, pack8<In>(y), buf);
         if (OUT == kOutMX) {
             uint32_t byte;
-            const uint32_t c = mx4_encode<kMXFP4>(y, amax_bits8(y), n.nv, &byte);
+            const uint32_t c = mx4_encode<kMXFP4, false>(y, amax_bits8(y), n.nv, &byte);
             mx4_store<kMXFP4>(to, v, c, byte);
         }
     }
     if (OUT == kOutNV) {
         uint32_t byte;
-        const uint32_t c = mx4_encode<kNVFP4>(t, amax_bits8(t), n.nv, &byte);
+        const uint32_t c = mx4_encode<kNVFP4, true>(t, amax_bits8(t), n.nv, &byte);
         mx4_store<kNVFP4>(to, v, c, byte);
     }
     if (OUT <= kOutINT8) {
@@ -278,6 +279,128 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) k_norm_rows(const NormArgs 
 #pragma unroll
             for (int j = 0; j < 4; ++j) t.p[j] = mul2(t.p[j], w.p[j]);
             emit8<In, OUT, VEC>(a, row, v, to, t, n, buf);
+        }
+    }
+}
+
+// Dense rows of a width that is not a multiple of 8, 8-bit output: all tensors are
+// equally far off a 16-byte boundary (a.shift0 columns, more with every row), so
+// the columns are cut into vectors where memory is: vector v of a row that lies
+// s columns behind a boundary holds columns [8v - s, 8v - s + 8), whole words of every
+// tensor, codes included, but for the row's ends.  Only the weight is read through
+// a window.  (1021 x 5003 fp32: 12.3 us one column a lane.)
+template <class In>
+__device__ __forceinline__ Raw8<In> load_cut(const In* row, int c0, int cols) {
+    Raw8<In> r;
+    if (c0 >= 0 && c0 + 8 <= cols) {
+#pragma unroll
+        for (int j = 0; j < static_cast<int>(sizeof(In) / 2); ++j) r.q[j] = reinterpret_cast<const uint4*>(row + c0)[j];
+        return r;
+    }
+    F8 f{};
+    float e[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        const int c = c0 + k;
+        e[k] = c < 0 || c >= cols ? 0.0f : (sizeof(In) == 4 ? reinterpret_cast<const float*>(row)[c]
+                                                            : bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(row)[c]));
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) f.p[k] = make_float2(e[2 * k], e[2 * k + 1]);
+    return pack8<In>(f);
+}
+template <class In>
+__device__ __forceinline__ void store_cut(In* row, int c0, int cols, const Raw8<In>& r) {
+    if (c0 >= 0 && c0 + 8 <= cols) {
+#pragma unroll
+        for (int j = 0; j < static_cast<int>(sizeof(In) / 2); ++j) reinterpret_cast<uint4*>(row + c0)[j] = r.q[j];
+        return;
+    }
+    const uint32_t w[8] = {r.q[0].x, r.q[0].y, r.q[0].z, r.q[0].w, r.q[sizeof(In) / 2 - 1].x, r.q[sizeof(In) / 2 - 1].y,
+                           r.q[sizeof(In) / 2 - 1].z, r.q[sizeof(In) / 2 - 1].w};
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        const int c = c0 + k;
+        if (c < 0 || c >= cols) continue;
+        if (sizeof(In) == 4) reinterpret_cast<uint32_t*>(row)[c] = w[k];
+        else reinterpret_cast<uint16_t*>(row)[c] = static_cast<uint16_t>(w[k / 2] >> (16 * (k & 1)));
+    }
+}
+// Eight columns of the weight from any column on.
+__device__ __forceinline__ F8 load_weight_cut(const void* w, int w_kind, int c0, int cols) {
+    if (w_kind & 1) return unpack8<uint16_t>([&] {
+        Raw8<uint16_t> r;
+        const uint16_t* p = static_cast<const uint16_t*>(w);
+        uint32_t e[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) e[k] = c0 + k < 0 || c0 + k >= cols ? 0u : __ldg(p + c0 + k);
+        r.q[0] = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
+        return r;
+    }());
+    const float* p = static_cast<const float*>(w);
+    float e[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) e[k] = c0 + k < 0 || c0 + k >= cols ? 0.0f : __ldg(p + c0 + k);
+    return F8{{{e[0], e[1]}, {e[2], e[3]}, {e[4], e[5]}, {e[6], e[7]}}};
+}
+
+template <class In, int OUT, int NV, bool SMALL>
+__global__ void __launch_bounds__(SMALL ? 320 : 1024, SMALL ? 4 : 1) k_norm_cut(const NormArgs a) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int width = blockDim.x, t0 = threadIdx.x;
+    int parity = 0;
+    for (long long rl = blockIdx.x; rl < a.rows; rl += gridDim.x, parity ^= 1) {
+        const int row = static_cast<int>(rl);
+        const int s = static_cast<int>((a.shift0 + rl * a.cols) & 7);
+        const size_t at = static_cast<size_t>(row) * a.cols;
+        const In* x = static_cast<const In*>(a.x) + row * a.x_stride;
+        Raw8<In> h[NV];
+#pragma unroll
+        for (int k = 0; k < NV; ++k) h[k] = load_cut<In>(x, 8 * (t0 + k * width) - s, a.cols);
+        if (a.res) {
+            const In* res = static_cast<const In*>(a.res) + row * a.res_stride;
+            Raw8<In> q[NV];
+#pragma unroll
+            for (int k = 0; k < NV; ++k) q[k] = load_cut<In>(res, 8 * (t0 + k * width) - s, a.cols);
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                h[k] = add8<In>(h[k], q[k]);
+                if (a.sum) store_cut<In>(static_cast<In*>(a.sum) + at, 8 * (t0 + k * width) - s, a.cols, h[k]);
+            }
+        }
+        float2 s2 = both(0.0f);
+        uint32_t tm = 0;
+        F8 t[NV];
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+            t[k] = row_terms(unpack8<In>(h[k]), load_weight_cut(a.w, a.w_kind, 8 * (t0 + k * width) - s, a.cols), s2, tm);
+        float ss = s2.x + s2.y;
+        block_sum_max(ss, tm, parity);
+        const RowNorm n = row_norm<OUT>(a, row, ss, tm, t0 == 0);
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int c0 = 8 * (t0 + k * width) - s;
+            if (a.y) {
+                F8 y;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) y.p[i] = mul2(t[k].p[i], both(n.r));
+                store_cut<In>(static_cast<In*>(a.y) + at, c0, a.cols, pack8<In>(y));
+            }
+            uint32_t c[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 q = mul2(t[k].p[i], both(n.to_code));
+                c[i] = ocp_encode2<OUT>(q.x, q.y);
+            }
+            uint8_t* o = a.codes + at;
+            if (c0 >= 0 && c0 + 8 <= a.cols) {
+                *reinterpret_cast<uint2*>(o + c0) = make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (c0 + e >= 0 && c0 + e < a.cols) o[c0 + e] = static_cast<uint8_t>(c[e / 2] >> (8 * (e & 1)));
+            }
         }
     }
 }
@@ -680,12 +803,33 @@ nq_status_t launch_norm_ring(const NormArgs& a, int nvec, const DeviceInfo& di, 
     return cuda_status(launch_pdl(kern, dim3(grid), dim3(threads), smem, s, a, stages, device_error_word()), who);
 }
 
+template <class In, int OUT, int NV, bool SMALL>
+nq_status_t launch_norm_cut(const NormArgs& a, int threads, const DeviceInfo& di, cudaStream_t s, const char* who) {
+    auto kern = k_norm_cut<In, OUT, NV, SMALL>;
+    int per_sm = 0;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, threads, 0) != cudaSuccess || per_sm < 1) {
+        cudaGetLastError();
+        per_sm = 1;
+    }
+    const int grid = static_cast<int>(std::min<long long>(a.rows, static_cast<long long>(di.sm_count) * per_sm));
+    return cuda_status(launch_pdl(kern, dim3(grid), dim3(threads), 0, s, a), who);
+}
+
 template <class In, int OUT, bool VEC>
 nq_status_t launch_norm(const NormArgs& a, const DeviceInfo& di, cudaStream_t s, const char* who) {
     constexpr int NVMAX = sizeof(In) == 2 ? 4 : 2;  // 64 bytes a thread of each tensor
     int nvec = (a.cols + 7) / 8;
     if (OUT == kOutMX) nvec = mx4_words(a.cols, 32) * 16;  // whole scale words
     if (OUT == kOutNV) nvec = mx4_words(a.cols, 16) * 8;
+    if constexpr (OUT <= kOutINT8 && !VEC) {
+        if (a.shift0 >= 0 && nvec + 1 <= 1024 * NVMAX) {
+            const int cut = nvec + 1;  // a row may begin inside its first vector
+            if (cut <= 256) return launch_norm_cut<In, OUT, 1, true>(a, (cut + 31) / 32 * 32, di, s, who);
+            const int threads = ((cut + NVMAX - 1) / NVMAX + 31) / 32 * 32;
+            if (sizeof(In) == 4 && threads <= 320) return launch_norm_cut<In, OUT, NVMAX, true>(a, threads, di, s, who);
+            return launch_norm_cut<In, OUT, NVMAX, false>(a, threads, di, s, who);
+        }
+    }
     if (nvec <= 32 * NVMAX) {
         if (nvec <= 32) return launch_norm_rows<In, OUT, VEC, 1, true>(a, 256, di, s, who);
         return launch_norm_rows<In, OUT, VEC, NVMAX, true>(a, 256, di, s, who);
@@ -740,8 +884,13 @@ nq_status_t norm_impl(const char* who, const nq_rmsnorm_desc_t* d, const void* x
     const size_t es = d->dtype == NQ_BF16 ? 2 : 4;
     const bool vec = d->cols % 8 == 0 && strided_ok(xs, es) && (!residual || strided_ok(rs, es)) && aligned16(x) &&
                      aligned16(residual) && aligned16(sum) && aligned16(y) && aligned16(codes);
+    // the tensors' common distance from a boundary of 8 columns, row for row
+    auto off = [&](const void* p, size_t e) { return static_cast<int>(reinterpret_cast<uintptr_t>(p) / e % 8); };
+    const bool agree = xs % 8 == static_cast<size_t>(d->cols) % 8 && (!residual || rs % 8 == static_cast<size_t>(d->cols) % 8) &&
+                       (!residual || off(residual, es) == off(x, es)) && (!sum || off(sum, es) == off(x, es)) &&
+                       (!y || off(y, es) == off(x, es)) && codes && off(codes, 1) == off(x, es);
     const NormArgs a{x, residual, weight, sum, y, codes, bscales, scales, d->rows, d->cols, xs, rs, d->eps, 1.0f / d->cols,
-                     (d->weight_dtype == NQ_BF16 ? 1 : 0) | (aligned16(weight) ? 2 : 0)};
+                     (d->weight_dtype == NQ_BF16 ? 1 : 0) | (aligned16(weight) ? 2 : 0), agree ? off(x, es) : -1};
     const bool bf = d->dtype == NQ_BF16;
     switch (out) {
         case kOutE4M3: return norm_out<kOutE4M3>(a, bf, vec, di, s, who);
@@ -768,7 +917,9 @@ nq_status_t launch_grad(const GradArgs& a, float* dw, const DeviceInfo& di, cuda
     size_t smem = 0;
     if (VEC) {
         // two to four rows ahead, about 40 KB of them a block
-        const size_t row = static_cast<size_t>(a.cols) * sizeof(In) * (a.dsum && a.dx ? 3 : 2);
+        // (room for dsum even where dx is not asked for: the grid, and with it the order of
+        // the weight gradient's sum, does not depend on dx)
+        const size_t row = static_cast<size_t>(a.cols) * sizeof(In) * (a.dsum ? 3 : 2);
         stages = static_cast<int>(std::max<size_t>(2, std::min<size_t>(4, 60 * 1024 / row)));
         if (stages * row > kGradSmem) stages = 1;
         smem = stages * (row + 8);

@@ -2,13 +2,7 @@
 references (tests/mx4_ref.py).
 
 Tolerances:
-- quantize: MXFP4 divides by powers of two, so codes and scales are the
-  reference's, value for value.  NVFP4 of bf16 values too (borders of ratios of
-  small integers stay borders).  NVFP4 of fp32 values: a block scale may move to
-  the neighbour where 448 amax / A is within 2^-20 of a border (the grid of 20
-  mantissa bits the kernel rounds it to, half a step of 2^-21, plus two fp32
-  roundings of 2^-24), and a code where its quotient is within 2^-17 of one (the
-  grid of 2^-17, half a step of 2^-18, plus 2^-21.4 of at most 9).
+- quantize: codes and scales are the correctly rounded ones, value for value.
 - dequantize: exact products rounded to fp32 once (2^-24), to bf16 once more (2^-8 eps / 2).
 - product: every product of two elements and two scales is exact; a group of 64
   is summed by one instruction and added to the fp32 accumulator, each to
@@ -62,35 +56,24 @@ def quantize(nq, x, fmt, stride=0, stream=None):
     return codes, scales, g
 
 
-def check_quantized(x, codes, scales, g, fmt, loose):
+def check_quantized(x, codes, scales, g, fmt):
     """Packed results (numpy, without guards) against the reference for doubles x."""
     rows, cols = x.shape
     q, s, gr = R.quantize(x, fmt)
     nb = (cols + R.BLOCK[fmt] - 1) // R.BLOCK[fmt]
     got_s = R.unpack_scales(scales, rows, cols, fmt)
-    pad = 2.0 ** -127 if fmt == R.MX else 0.0
-    assert np.all(got_s[:, nb:] == pad), "scales behind the last block"
-    same = got_s == s
-    if loose and not same.all():
-        top = np.abs(R.blocks(x, fmt)).max(-1)
-        v = 448.0 * top / np.maximum(top.max(1, keepdims=True), 2688.0 * 2.0 ** -110)
-        lo, hi = R.e4m3(v * (1 - 2.0 ** -20)), R.e4m3(v * (1 + 2.0 ** -20))
-        assert np.all(same | (got_s == lo) | (got_s == hi))
-    else:
-        assert same.all(), "block scales"
+    assert np.all(got_s[:, nb:] == (2.0 ** -127 if fmt == R.MX else 0.0)), "scales behind the last block"
+    assert np.array_equal(got_s, s), "block scales"
     if fmt == R.NV:
         assert np.array_equal(g, gr.astype(np.float32)), "row scales"
     got = R.unpack_codes(codes, rows, cols)
     assert np.all(got[:, cols:] == 0), "codes behind the last column"
     w = q.shape[1] * q.shape[2]
-    got = np.pad(got, ((0, 0), (0, w - got.shape[1]))).reshape(q.shape) if w > got.shape[1] else got[:, :w].reshape(q.shape)
-    ok = got == R.e2m1(q)
-    if loose:
-        ok |= (got == R.e2m1(q - 2.0 ** -17)) | (got == R.e2m1(q + 2.0 ** -17))
-    assert ok[same].all(), "codes"
+    got = np.pad(got, ((0, 0), (0, max(0, w - got.shape[1]))))[:, :w].reshape(q.shape)
+    assert np.array_equal(got, R.e2m1(q)), "codes"
 
 
-SHAPES = [(1, 1), (1, 64), (2, 15), (3, 16), (5, 17), (7, 33), (33, 128), (129, 130), (4, 1000), (300, 511), (64, 4096),
+SHAPES = [(1, 1), (1, 64), (70, 496), (900, 16), (700, 2064), (40, 512), (2, 15), (3, 16), (5, 17), (7, 33), (33, 128), (129, 130), (4, 1000), (300, 511), (64, 4096),
           (2, 8192), (3, 8200), (2, 16384), (2, 20008), (1, 40000), (3, 33001)]
 
 
@@ -116,7 +99,7 @@ def test_quantize(nq, fmt, bf16, shape):
     if g is not None:
         assert np.all(g[rows:].cpu().numpy() == -7.0)
         g = g[:rows].cpu().numpy()
-    check_quantized(x.double().cpu().numpy(), codes[:n], scales[:m], g, fmt, loose=fmt == R.NV and not bf16)
+    check_quantized(x.double().cpu().numpy(), codes[:n], scales[:m], g, fmt)
 
 
 @pytest.mark.parametrize("fmt", FMTS)
@@ -129,7 +112,26 @@ def test_quantize_borders(nq, fmt):
     assert np.array_equal(t.double().cpu().numpy(), x)
     codes, scales, g = quantize(nq, t, fmt)
     n, m = 200 * nq.mx4_row_bytes(1600), nq.mx4_scale_bytes(200, 1600, fmt)
-    check_quantized(x, codes[:n].cpu().numpy(), scales[:m].cpu().numpy(), None if g is None else g[:200].cpu().numpy(), fmt, False)
+    check_quantized(x, codes[:n].cpu().numpy(), scales[:m].cpu().numpy(), None if g is None else g[:200].cpu().numpy(), fmt)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_quantize_fp32_next_to_borders(nq, fmt):
+    """fp32 values a step or two of 2^-24 from a border of their code, on either side and on it."""
+    import torch
+    rng = np.random.default_rng(5)
+    rows, cols = 400, 640
+    level = rng.uniform(1.0, 2.0, (rows, 1)).astype(np.float32).astype(np.float64)
+    s = R.e4m3(rng.uniform(1.0, 448.0, (rows, cols // 16, 1)))
+    mids = np.array([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0])
+    x = (rng.choice(mids, (rows, cols // 16, 16)) * s * level[..., None] / 2688.0).reshape(rows, cols).astype(np.float32)
+    x = (x.view(np.int32) + rng.integers(-2, 3, x.shape, dtype=np.int32)).view(np.float32) * rng.choice([-1.0, 1.0], x.shape).astype(np.float32)
+    x[:, ::16] = (s[..., 0] * level / 448.0).astype(np.float32)   # the blocks' maxima, near borders of the scales
+    x[:, 0] = level[:, 0]
+    t = torch.from_numpy(x).cuda()
+    codes, scales, g = quantize(nq, t, fmt)
+    n, m = rows * nq.mx4_row_bytes(cols), nq.mx4_scale_bytes(rows, cols, fmt)
+    check_quantized(x.astype(np.float64), codes[:n].cpu().numpy(), scales[:m].cpu().numpy(), None if g is None else g[:rows].cpu().numpy(), fmt)
 
 
 @pytest.mark.parametrize("fmt", FMTS)
@@ -141,7 +143,7 @@ def test_quantize_extreme_magnitudes(nq, fmt, scale):
     codes, scales, g = quantize(nq, x, fmt)
     n, m = 9 * nq.mx4_row_bytes(160), nq.mx4_scale_bytes(9, 160, fmt)
     check_quantized(x.double().cpu().numpy(), codes[:n].cpu().numpy(), scales[:m].cpu().numpy(),
-                    None if g is None else g[:9].cpu().numpy(), fmt, loose=fmt == R.NV)
+                    None if g is None else g[:9].cpu().numpy(), fmt)
 
 
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
