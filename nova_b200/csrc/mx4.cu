@@ -289,13 +289,8 @@ struct QuantArgs {
 template <class In, int F, bool VEC, int NV, bool WARP>
 nq_status_t launch_quant(const In* src, const QuantArgs& a, int threads, const DeviceInfo& di, cudaStream_t s) {
     auto kern = k_mx4_quant<In, F, VEC, NV, WARP>;
-    int per_sm = 0;
-    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, threads, 0) != cudaSuccess || per_sm < 1) {
-        cudaGetLastError();
-        per_sm = 1;
-    }
     const long long blocks = WARP ? (static_cast<long long>(a.rows) + threads / 32 - 1) / (threads / 32) : a.rows;
-    const int grid = static_cast<int>(std::min<long long>(blocks, static_cast<long long>(di.sm_count) * per_sm));
+    const int grid = persistent_grid(kern, threads, 0, blocks, di);
     return cuda_status(launch_pdl(kern, dim3(grid), dim3(threads), 0, s, src, a.ld, a.codes, a.bscales, a.rscales, a.rows, a.cols),
                        "nq_quantize_rows_mx4");
 }
@@ -303,13 +298,8 @@ nq_status_t launch_quant(const In* src, const QuantArgs& a, int threads, const D
 template <class In, int F, int NV, bool WARP>
 nq_status_t launch_quant16(const In* src, const QuantArgs& a, int threads, const DeviceInfo& di, cudaStream_t s) {
     auto kern = k_mx4_quant16<In, F, NV, WARP>;
-    int per_sm = 0;
-    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, threads, 0) != cudaSuccess || per_sm < 1) {
-        cudaGetLastError();
-        per_sm = 1;
-    }
     const long long blocks = WARP ? (static_cast<long long>(a.rows) + threads / 32 - 1) / (threads / 32) : a.rows;
-    const int grid = static_cast<int>(std::min<long long>(blocks, static_cast<long long>(di.sm_count) * per_sm));
+    const int grid = persistent_grid(kern, threads, 0, blocks, di);
     return cuda_status(launch_pdl(kern, dim3(grid), dim3(threads), 0, s, src, a.ld, a.codes, a.bscales, a.rscales, a.rows, a.cols),
                        "nq_quantize_rows_mx4");
 }

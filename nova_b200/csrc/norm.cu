@@ -767,13 +767,8 @@ nq_status_t check_desc(const char* who, const nq_rmsnorm_desc_t* d, size_t* xs, 
 template <class In, int OUT, bool VEC, int NV, bool WARP>
 nq_status_t launch_norm_rows(const NormArgs& a, int threads, const DeviceInfo& di, cudaStream_t s, const char* who) {
     auto kern = k_norm_rows<In, OUT, VEC, NV, WARP>;
-    int per_sm = 0;
-    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, threads, 0) != cudaSuccess || per_sm < 1) {
-        cudaGetLastError();
-        per_sm = 1;
-    }
     const long long blocks = WARP ? (static_cast<long long>(a.rows) + threads / 32 - 1) / (threads / 32) : a.rows;
-    const int grid = static_cast<int>(std::min<long long>(blocks, static_cast<long long>(di.sm_count) * per_sm));
+    const int grid = persistent_grid(kern, threads, 0, blocks, di);
     return cuda_status(launch_pdl(kern, dim3(grid), dim3(threads), 0, s, a), who);
 }
 
@@ -794,24 +789,14 @@ nq_status_t launch_norm_ring(const NormArgs& a, int nvec, const DeviceInfo& di, 
         return NQ_SUCCESS;
     });
     if (st != NQ_SUCCESS) return st;
-    int per_sm = 0;
-    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, threads, smem) != cudaSuccess || per_sm < 1) {
-        cudaGetLastError();
-        per_sm = 1;
-    }
-    const int grid = static_cast<int>(std::min<long long>(a.rows, static_cast<long long>(di.sm_count) * per_sm));
+    const int grid = persistent_grid(kern, threads, smem, a.rows, di);
     return cuda_status(launch_pdl(kern, dim3(grid), dim3(threads), smem, s, a, stages, device_error_word()), who);
 }
 
 template <class In, int OUT, int NV, bool SMALL>
 nq_status_t launch_norm_cut(const NormArgs& a, int threads, const DeviceInfo& di, cudaStream_t s, const char* who) {
     auto kern = k_norm_cut<In, OUT, NV, SMALL>;
-    int per_sm = 0;
-    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, threads, 0) != cudaSuccess || per_sm < 1) {
-        cudaGetLastError();
-        per_sm = 1;
-    }
-    const int grid = static_cast<int>(std::min<long long>(a.rows, static_cast<long long>(di.sm_count) * per_sm));
+    const int grid = persistent_grid(kern, threads, 0, a.rows, di);
     return cuda_status(launch_pdl(kern, dim3(grid), dim3(threads), 0, s, a), who);
 }
 
@@ -932,12 +917,7 @@ nq_status_t launch_grad(const GradArgs& a, float* dw, const DeviceInfo& di, cuda
         });
         if (st != NQ_SUCCESS) return st;
     }
-    int per_sm = 0;
-    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, threads, smem) != cudaSuccess || per_sm < 1) {
-        cudaGetLastError();
-        per_sm = 1;
-    }
-    const int grid = static_cast<int>(std::min<long long>(a.rows, static_cast<long long>(di.sm_count) * per_sm));
+    const int grid = persistent_grid(kern, threads, smem, a.rows, di);
     void* part = nullptr;
     nq_status_t st = NQ_SUCCESS;
     if (dw) st = scratch_alloc(&part, static_cast<size_t>(grid) * a.cols * 4, s);

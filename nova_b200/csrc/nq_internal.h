@@ -47,6 +47,19 @@ cudaError_t launch_pdl(void (*kern)(P...), dim3 grid, dim3 block, size_t smem, c
     return cudaLaunchKernelEx(&cfg, kern, std::forward<A>(args)...);
 }
 
+// Blocks of a persistent kernel: as many as are resident at once, at most `work`.
+template <class K>
+int persistent_grid(K kern, int threads, size_t smem, long long work, const DeviceInfo& di) {
+    if (work <= di.sm_count) return static_cast<int>(work);
+    int per_sm = 0;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, threads, smem) != cudaSuccess || per_sm < 1) {
+        cudaGetLastError();
+        per_sm = 1;
+    }
+    const long long most = static_cast<long long>(di.sm_count) * per_sm;
+    return static_cast<int>(work < most ? work : most);
+}
+
 // Stream-ordered scratch from a library-owned memory pool of the current
 // device: cudaMallocAsync after the first call on a device reuses the pool's
 // cached blocks instead of reaching the driver.

@@ -394,3 +394,68 @@ def test_linear_captured_and_replayed(nq, fmt, m):
     layers[0].run()
     torch.cuda.synchronize()
     assert torch.equal(layers[0].out, refs[2]) and nq.device_error_flags() == 0
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_shared_out_product_captured_and_replayed(nq, fmt):
+    """Few rows against a long K (k-blocks of a unit on several CTAs, parts through a workspace): two graphs
+    replayed at once beside eager calls give the eager result."""
+    import torch
+    m, n, k = 4, 4096, 28672
+    w = make(n, k, 1, True, 0.02)
+    b = buffers(nq, n, k, fmt, 0)
+    x = make(m, k, 2, True)
+    a = buffers(nq, m, k, fmt, 0)
+    s = torch.cuda.current_stream().cuda_stream
+    for t, q, rows in ((w, b, n), (x, a, m)):
+        nq.quantize_rows_mx4(t.data_ptr(), nq.BF16, 0, q[0].data_ptr(), q[1].data_ptr(), q[2].data_ptr() if q[2] is not None else 0,
+                             rows, k, fmt, s)
+    a, b = [(q[0], q[1], None if q[2] is None else q[2][:r].contiguous()) for q, r in ((a, m), (b, n))]
+    ref = product(nq, a, b, m, n, k, fmt, False)
+    va, vb = (R.values(q[0].cpu().numpy(), q[1].cpu().numpy(), r, k, fmt) for q, r in ((a, m), (b, n)))
+    check_product(ref, va, vb, a, b, k, False)
+    outs = [torch.full_like(ref, 99.0) for _ in range(3)]
+    graphs = []
+    for o in outs[:2]:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            for _ in range(3):
+                product(nq, a, b, m, n, k, fmt, False, out=o)
+        graphs.append(g)
+    side = torch.cuda.Stream()
+    for _ in range(4):
+        for o in outs:
+            o.fill_(99.0)
+        torch.cuda.synchronize()
+        graphs[0].replay()
+        with torch.cuda.stream(side):
+            graphs[1].replay()
+        product(nq, a, b, m, n, k, fmt, False, out=outs[2])
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, ref) for o in outs)
+    assert nq.device_error_flags() == 0
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_quantize_past_32_bits(nq, fmt):
+    """More than 2^32 bytes of input and 2^31 elements: the last rows equal the same rows quantized alone."""
+    import torch
+    rows, cols, tail = 36000, 65536, 300
+    x = torch.empty(rows, cols, dtype=torch.bfloat16, device="cuda")
+    for r in range(0, rows, 4000):
+        x[r:r + 4000] = make(min(4000, rows - r), cols, r, True)
+    codes, scales, g = quantize(nq, x, fmt)
+    first = rows // 128 * 128 - 256
+    cc, ss, gg = quantize(nq, x[first:], fmt)
+    n, pitch = rows - first, nq.mx4_row_bytes(cols)
+    assert torch.equal(codes[first * pitch:rows * pitch], cc[:n * pitch])
+    at = first // 128 * R.words(cols, fmt) * 512
+    idx = torch.from_numpy(R.scale_index(n, cols, fmt)).cuda()
+    assert torch.equal(scales[at:][idx], ss[idx])
+    if g is not None:
+        assert torch.equal(g[first:rows], gg[:n])
+    out = torch.empty(rows, cols, dtype=torch.bfloat16, device="cuda")
+    nq.dequantize_rows_mx4(codes.data_ptr(), scales.data_ptr(), g.data_ptr() if g is not None else 0, out.data_ptr(), nq.BF16, rows, cols,
+                           fmt, torch.cuda.current_stream().cuda_stream)
+    assert torch.equal(out[first:], dequantize(nq, cc, ss, gg, n, cols, fmt, True))
+    assert (out[first:].float() - x[first:].float()).norm() < 0.2 * x[first:].float().norm()

@@ -380,3 +380,48 @@ def test_norm_to_product_layer(nq, tokens):
     assert torch.all((out.double() - ref).abs() <= ref.abs() * (2.0 ** -8 + 4 * U) + 1e-30)
     assert ((out.double() - exact).norm() / exact.norm()).item() < 0.03
     assert nq.device_error_flags() == 0
+
+
+def test_norm_past_32_bits(nq):
+    """More than 2^31 elements: the last rows equal the same rows alone, forward and backward."""
+    import torch
+    rows, cols = 270000, 8192
+    x = torch.empty(rows, cols, dtype=torch.bfloat16, device="cuda")
+    for r in range(0, rows, 30000):
+        x[r:r + 30000] = rand(min(30000, rows - r), cols, r, True)
+    w = rand(1, cols, 1, True).view(-1)
+    last = slice(rows - 1000, rows)
+    y, codes, _, scales = run(nq, x, None, w, E4M3, want_y=False)
+    _, c, _, sc = run(nq, x[last], None, w, E4M3, want_y=False)
+    assert torch.equal(codes[last], c) and torch.equal(scales[last], sc)
+    del codes, scales
+    dx = torch.empty_like(x)
+    s = torch.cuda.current_stream().cuda_stream
+    d = nq.make_rmsnorm_desc(rows, cols, nq.BF16, nq.BF16, EPS)
+    nq.rmsnorm_backward(C.byref(d), ptr(x), ptr(w), ptr(x), 0, ptr(dx), 0, s)
+    dx1 = torch.empty(1000, cols, dtype=torch.bfloat16, device="cuda")
+    d = nq.make_rmsnorm_desc(1000, cols, nq.BF16, nq.BF16, EPS)
+    xl = x[last].clone()
+    nq.rmsnorm_backward(C.byref(d), ptr(xl), ptr(w), ptr(xl), 0, ptr(dx1), 0, s)
+    assert torch.equal(dx[last], dx1)
+
+
+@pytest.mark.parametrize("bf16", [True, False])
+def test_dense_unaligned_base(nq, bf16):
+    """Dense odd-width rows whose tensors start off a 16-byte boundary, all by the same or by different distances."""
+    import torch
+    rows, cols = 37, 1003
+    n = rows * cols
+    flat = lambda seed, off: rand(1, n + 8, seed, bf16).view(-1)[off:off + n].view(rows, cols)
+    w = rand(1, cols, 9, bf16).view(-1)
+    for offs in ((0, 0, 0), (3, 3, 3), (3, 1, 0), (8, 0, 5)):
+        x, res = flat(1, offs[0]), flat(2, offs[1])
+        whole = torch.full((n + 16,), 7.0, dtype=x.dtype, device="cuda")
+        sm = whole[offs[2]:offs[2] + n].view(rows, cols)
+        y, codes, _, scales = run(nq, x, res, w, E4M3, sum=sm)
+        h = reference_h(x, res)
+        assert np.array_equal(sm.double().cpu().numpy(), h)
+        assert torch.all(whole[:offs[2]] == 7.0) and torch.all(whole[offs[2] + n:] == 7.0)
+        t, r = R.rmsnorm(h, w.double().cpu().numpy(), EPS)
+        check_y(y, t, r, cols)
+        check_codes8(codes, scales, t, r, cols, E4M3)
