@@ -8,8 +8,8 @@
 // k_mx4_pair (more than 64 rows): a cluster of two CTAs computes 256 x 256
 //   tiles with cta_group::2, persistent, banded tile order.
 // k_mx4_decode (up to 64 rows): operands swapped -- 128 rows of B are the MMA's
-//   M side, the rows of A its N side -- and B's k-blocks cut into one
-//   contiguous range a CTA, so every SM streams the same number of bytes.
+//   M side, the rows of A its N side; units of 128 rows whole, or their k-blocks
+//   shared out so that every SM streams the same number of bytes.
 #include <algorithm>
 #include <atomic>
 #include <cstring>
@@ -63,6 +63,16 @@ __global__ void __launch_bounds__(256) k_mx4_empty(int M, int N, MxEpi ep) {
 }
 
 // ---------------- CTA pair, 256 x 256 tiles ----------------
+// Bound by the tensor pipe and, run back to back, by the board's power: 4096^3
+// MXFP4 27.4 us (5.0 PFLOP/s), 8192^3 NVFP4 194 us (5.7 PFLOP/s, tensor pipe 74%
+// active, DRAM traffic 211 MB of 210), 8192 x 14336 x 4096 NVFP4 218 us (4.4
+// PFLOP/s) for seconds on end, with SM clocks at 1.46 GHz under the cap.  Of those
+// 218 us the operands' way into shared memory and the epilogue take about 30 each
+// (the MMAs alone, on data already there: 161); the accumulators' handover between
+// tiles takes about 1600 cycles of a tile's 10800.  Tiles of 256 x 192 with two whole
+// accumulators hide that, but load 19% more and end at the same time (211 against
+// 210 us, MXFP4) at a lower clock; stores from registers instead of
+// staged TMA stores measured the same.
 template <bool MX, bool BF16>
 struct PairCfg {
     static constexpr int WORDS = MX ? 2 : 4;          // scale words (tiles) a stage
@@ -419,6 +429,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<MX, BF16>::T
 // every time.  Ranges go to the CTAs in reverse, so an owner waits for CTAs of
 // lower index only: those are placed before it, and a grid that shares the GPU
 // with another one still finishes.
+// Bound by HBM where B is large: 16 x 28672 x 8192 NVFP4 23.8 us, 5.6 TB/s of B's
+// codes and scales (85% of the measured copy rate; 64 rows 26.8 us).  What is missing: the first
+// loads' latency, SMs that finish up to 3 us apart, the last epilogue.
 template <bool MX, int BT>
 struct DecodeCfg {
     static constexpr int WORDS = MX ? 2 : 4;
