@@ -125,6 +125,9 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) k_mx4_quant16(const In* __r
     const int width = WARP ? 32 : blockDim.x;
     const int t0 = WARP ? lane_of() : threadIdx.x;
     const int per = WARP ? blockDim.x >> 5 : 1;
+    // few rows: their first bytes to L2 (which is coherent) while the kernel before ends (with a 1 x 8192 x
+    // 8192 product behind it 14.3 -> 13.4 us)
+    if (NV == 1 && !WARP && blockIdx.x < rows && t0 < nvec) prefetch_l2(src + blockIdx.x * ld + 16 * t0);
     pdl_wait();
     int parity = 0;
     for (long long rl = static_cast<long long>(blockIdx.x) * per + (WARP ? threadIdx.x >> 5 : 0); rl < rows;

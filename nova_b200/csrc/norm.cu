@@ -10,8 +10,8 @@
 //
 // Which kernel: rows in registers (k_norm_rows: a warp or a block a row); many
 // aligned rows through a bulk-copy ring (k_norm_ring: 16384 x 8192 bf16 with
-// residual, E4M3: 154 us, 6.1 TB/s, against 165 from registers; 16384 columns lose by it, 298 against 286);
-// dense rows of odd widths cut where memory is (k_norm_cut: 16384 x 5003 bf16 118 us
+// residual, E4M3: 154 us, 6.1 TB/s, against 165 from registers; 16384 columns lose
+// by it, 298 against 286); dense rows of odd widths cut where memory is (k_norm_cut: 16384 x 5003 bf16 118 us
 // against 187); rows too wide for registers in two passes.  One row: 2.6 us a launch
 // in a graph.  The gradient: 8192 x 4096 bf16 51 us (5.2 TB/s), of which the partial
 // rows' sum takes 4.5.
@@ -244,6 +244,12 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) k_norm_rows(const NormArgs 
     const int width = WARP ? 32 : blockDim.x;
     const int t0 = WARP ? threadIdx.x & 31 : threadIdx.x;
     const int per = WARP ? blockDim.x >> 5 : 1;  // rows a block takes at once
+    if (VEC && NV == 1 && !WARP && blockIdx.x < a.rows && 8 * t0 < a.cols) {
+        // few rows: their first bytes to L2 (which is coherent) while the kernel before ends
+        prefetch_l2(static_cast<const In*>(a.x) + blockIdx.x * a.x_stride + 8 * t0);
+        if (a.res) prefetch_l2(static_cast<const In*>(a.res) + blockIdx.x * a.res_stride + 8 * t0);
+        prefetch_l2(static_cast<const uint8_t*>(a.w) + ((a.w_kind & 1) ? 16 : 32) * static_cast<size_t>(t0));
+    }
     pdl_wait();
     int parity = 0;
     for (long long rl = static_cast<long long>(blockIdx.x) * per + (WARP ? threadIdx.x >> 5 : 0); rl < a.rows;

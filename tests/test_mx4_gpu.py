@@ -459,3 +459,52 @@ def test_quantize_past_32_bits(nq, fmt):
                            fmt, torch.cuda.current_stream().cuda_stream)
     assert torch.equal(out[first:], dequantize(nq, cc, ss, gg, n, cols, fmt, True))
     assert (out[first:].float() - x[first:].float()).norm() < 0.2 * x[first:].float().norm()
+
+
+def test_two_threads_at_once(nq):
+    """Two host threads, each with its stream, buffers and shapes, through quantize and every kind of product."""
+    import threading
+    import torch
+    jobs = [(R.NV, [(4, 4096, 14336), (300, 1000, 1024), (40, 2048, 512)]), (R.MX, [(16, 8192, 8192), (70, 700, 640), (2, 512, 16384)])]
+    failed = []
+
+    def work(fmt, shapes):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                layers = []
+                for m, n, k in shapes:
+                    w, x = make(n, k, m + n, True, 0.02), make(m, k, k, True)
+                    b, a = buffers(nq, n, k, fmt, 0), buffers(nq, m, k, fmt, 0)
+                    s = stream.cuda_stream
+                    p = lambda t: t.data_ptr() if t is not None else 0
+                    nq.quantize_rows_mx4(w.data_ptr(), nq.BF16, 0, p(b[0]), p(b[1]), p(b[2]), n, k, fmt, s)
+                    layers.append((m, n, k, x, a, b, w))
+
+                def step(m, n, k, x, a, b):
+                    nq.quantize_rows_mx4(x.data_ptr(), nq.BF16, 0, p(a[0]), p(a[1]), p(a[2]), m, k, fmt, s)
+                    return product(nq, a, b, m, n, k, fmt, False, stream=s)
+
+                refs = []
+                for l in layers:
+                    refs.append(step(*l[:6]))
+                    stream.synchronize()
+                for _ in range(30):
+                    outs = [step(*l[:6]) for l in layers]
+                    stream.synchronize()
+                    if not all(torch.equal(o, r) for o, r in zip(outs, refs)):
+                        failed.append(fmt)
+                for (m, n, k, x, _, _, w), r in zip(layers, refs):
+                    want = x.double() @ w.double().t()
+                    if ((r[:m * n].view(m, n) - want).norm() / want.norm()).item() > 0.25:
+                        failed.append((m, n, k))
+        except Exception as e:
+            failed.append(repr(e))
+
+    threads = [threading.Thread(target=work, args=j) for j in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(120)
+    torch.cuda.synchronize()
+    assert not failed and nq.device_error_flags() == 0
