@@ -3,7 +3,7 @@
 // Aligned rows with 16 columns a lane: 28672 x 8192 bf16 to MXFP4 96 us, to NVFP4
 // 91 us (6.2 and 6.6 TB/s), back to bf16 100 and 104 us (5.9 TB/s); 8192 x 4096
 // 15.0 and 15.5 us.  With 8 columns a lane NVFP4 took 113 us and the way back 116.
-// Unaligned rows move one column a lane (16384 x 4111 bf16 to NVFP4 63 us).
+// Unaligned rows move one column a lane (16384 x 4111 bf16 to NVFP4 55 us).
 #include <algorithm>
 #include <string>
 
@@ -181,7 +181,7 @@ __global__ void __launch_bounds__(kThreads) k_mx4_dequant16(const uint8_t* __res
     const int nvec = cols / 16;
     const int words = mx4_words(cols, Mx4Traits<F>::block);
     const int t0 = threadIdx.x % width;
-    const int per = kThreads / width;
+    const int per = blockDim.x / width;
     pdl_wait();
     for (long long rl = static_cast<long long>(blockIdx.x) * per + threadIdx.x / width; rl < rows;
          rl += static_cast<long long>(gridDim.x) * per) {
@@ -240,7 +240,7 @@ __global__ void __launch_bounds__(kThreads) k_mx4_dequant(const uint8_t* __restr
     const int nvec = (cols + 7) / 8;
     const int words = mx4_words(cols, Mx4Traits<F>::block);
     const int t0 = threadIdx.x % width;
-    const int per = kThreads / width;
+    const int per = blockDim.x / width;
     pdl_wait();
     for (long long rl = static_cast<long long>(blockIdx.x) * per + threadIdx.x / width; rl < rows;
          rl += static_cast<long long>(gridDim.x) * per) {
@@ -330,7 +330,10 @@ nq_status_t quant_impl(const void* p, const QuantArgs& a, const DeviceInfo& di, 
     if (nvec <= 32) return launch_quant<In, F, VEC, 1, true>(src, a, 256, di, s);
     if (nvec <= 32 * NVMAX) return launch_quant<In, F, VEC, NVMAX, true>(src, a, 256, di, s);
     if (a.rows < 2 * di.sm_count && nvec <= 1024) return launch_quant<In, F, VEC, 1, false>(src, a, (nvec + 31) / 32 * 32, di, s);
-    const int threads = ((nvec + NVMAX - 1) / NVMAX + 31) / 32 * 32;
+    // the most vectors a thread, or half of them where that leaves fewer lanes idle
+    auto lanes = [&](int nv) { return ((nvec + nv - 1) / nv + 31) / 32 * 32; };
+    const int threads = lanes(NVMAX), half = lanes(NVMAX / 2);
+    if (half <= 512 && half * (NVMAX / 2) < threads * NVMAX) return launch_quant<In, F, VEC, NVMAX / 2, false>(src, a, half, di, s);
     if (threads <= 1024) return launch_quant<In, F, VEC, NVMAX, false>(src, a, threads, di, s);
     const int grid = static_cast<int>(std::min<long long>(a.rows, static_cast<long long>(di.sm_count) * 8));
     return cuda_status(launch_pdl(k_mx4_quant_wide<In, F, VEC>, dim3(grid), dim3(kThreads), 0, s, src, a.ld, a.codes, a.bscales,
@@ -341,24 +344,19 @@ nq_status_t quant_impl(const void* p, const QuantArgs& a, const DeviceInfo& di, 
 template <class T, int F>
 nq_status_t dequant_impl(const uint8_t* codes, const uint8_t* bscales, const float* rscales, void* dst, int rows, int cols,
                          bool vec, const DeviceInfo& di, cudaStream_t s) {
-    const int nvec = (cols + 7) / 8;
-    int width = 32;
-    while (width < kThreads && 4 * width < nvec) width *= 2;
-    const long long blocks = (static_cast<long long>(rows) + kThreads / width - 1) / (kThreads / width);
-    const int grid = static_cast<int>(std::min<long long>(blocks, static_cast<long long>(di.sm_count) * 8));
-    if (cols % 16 == 0 && reinterpret_cast<uintptr_t>(dst) % 32 == 0) {
-        int w16 = 32;
-        while (w16 < kThreads && 8 * w16 < nvec) w16 *= 2;
-        const long long blocks16 = (static_cast<long long>(rows) + kThreads / w16 - 1) / (kThreads / w16);
-        const int grid16 = static_cast<int>(std::min<long long>(blocks16, static_cast<long long>(di.sm_count) * 8));
-        return cuda_status(launch_pdl(k_mx4_dequant16<T, F>, dim3(grid16), dim3(kThreads), 0, s, codes, bscales, rscales,
-                                      static_cast<T*>(dst), rows, cols, w16),
+    // `width` lanes a row with four vectors each (few rows: one each), as many rows as make a block of
+    // up to 256 threads
+    auto go = [&](auto kern, int nvec) {
+        const int width = std::min(kThreads, rows < 2 * di.sm_count ? (nvec + 31) / 32 * 32 : (nvec + 127) / 128 * 32);
+        const int per = kThreads / width;
+        const long long blocks = (static_cast<long long>(rows) + per - 1) / per;
+        const int grid = static_cast<int>(std::min<long long>(blocks, static_cast<long long>(di.sm_count) * 8));
+        return cuda_status(launch_pdl(kern, dim3(grid), dim3(width * per), 0, s, codes, bscales, rscales, static_cast<T*>(dst), rows,
+                                      cols, width),
                            "nq_dequantize_rows_mx4");
-    }
-    auto kern = vec ? k_mx4_dequant<T, F, true> : k_mx4_dequant<T, F, false>;
-    return cuda_status(launch_pdl(kern, dim3(grid), dim3(kThreads), 0, s, codes, bscales, rscales, static_cast<T*>(dst), rows, cols,
-                                  width),
-                       "nq_dequantize_rows_mx4");
+    };
+    if (cols % 16 == 0 && reinterpret_cast<uintptr_t>(dst) % 32 == 0) return go(k_mx4_dequant16<T, F>, cols / 16);
+    return go(vec ? k_mx4_dequant<T, F, true> : k_mx4_dequant<T, F, false>, (cols + 7) / 8);
 }
 
 }  // namespace
