@@ -11,7 +11,7 @@
 // Which kernel: rows in registers (k_norm_rows: a warp or a block a row); many
 // aligned rows through a bulk-copy ring (k_norm_ring: 16384 x 8192 bf16 with
 // residual, E4M3: 154 us, 6.1 TB/s, against 165 from registers; 16384 columns lose
-// by it, 298 against 286); dense rows of odd widths cut where memory is (k_norm_cut: 16384 x 5003 bf16 118 us
+// by it, 298 against 286); dense rows of odd widths cut where memory is (k_norm_cut: 16384 x 5003 bf16 130 us
 // against 187); rows too wide for registers in two passes.  One row: 2.6 us a launch
 // in a graph.  The gradient: 8192 x 4096 bf16 51 us (5.2 TB/s), of which the partial
 // rows' sum takes 4.5.
@@ -129,11 +129,21 @@ __device__ __forceinline__ void block_sum_max(float& s, uint32_t& m, int parity)
 // What a row's reduction gives the encoder.
 struct RowNorm {
     float r;        // 1 / rms (where it is needed: y, MXFP4)
-    float to_code;  // 8 bits: qmax / T
+    float tn, inv;  // 8 bits: T / 512 and its reciprocal
     NvRow nv;       // NVFP4
 };
 __device__ __forceinline__ float row_r(float sumsq, float inv_cols, float eps) {
     return rsqrtf(__fmaf_rn(sumsq, inv_cols, eps));
+}
+// The quotient t qmax / T of an 8-bit code, correctly rounded: a product with the
+// reciprocal, its remainder, one correction.  (Quotients of bf16 products are ratios of
+// small integers and fall on rounding borders; the product alone puts them to
+// either side.)
+template <int F>
+__device__ __forceinline__ float2 code_quotient(float2 t, const RowNorm& n) {
+    const float2 num = mul2(t, both(FmtTraits<F>::qmax / 512.0f));  // (scaled so that nothing overflows)
+    const float2 q = mul2(num, both(n.inv));
+    return fma2(fma2(q, both(-n.tn), num), both(n.inv), q);
 }
 // `first`: this thread stores the row's scale (the only place, besides y and
 // MXFP4, where r and its divisions are needed).
@@ -144,7 +154,8 @@ __device__ __forceinline__ RowNorm row_norm(const NormArgs& a, int row, float su
     if (OUT <= kOutINT8) {
         constexpr float qmax = FmtTraits<OUT <= kOutINT8 ? OUT : 0>::qmax;
         const float T = fmaxf(__uint_as_float(tmax), 0x1p-110f);
-        n.to_code = __fdiv_rn(qmax, T);
+        n.tn = T * 0x1p-9f;
+        n.inv = __frcp_rn(n.tn);
         if (first)
             a.scales[row] = tmax >= kInfBits ? __uint_as_float(0x7FC00000u)
                                              : (tmax == 0u ? 1.0f : __fdiv_rn(__fmul_rn(row_r(sumsq, a.inv_cols, a.eps), T), qmax));
@@ -180,7 +191,7 @@ __device__ __forceinline__ void emit8(const NormArgs& a, int row, int v, const M
         uint32_t c[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const float2 q = mul2(t.p[i], both(n.to_code));
+            const float2 q = code_quotient<F>(t.p[i], n);
             c[i] = ocp_encode2<F>(q.x, q.y);
         }
         store_codes8<VEC>(a.codes + static_cast<size_t>(row) * a.cols, v, a.cols, make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16)), buf);
@@ -404,7 +415,7 @@ __global__ void __launch_bounds__(SMALL ? 320 : 1024, SMALL ? 4 : 1) k_norm_cut(
             uint32_t c[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float2 q = mul2(t[k].p[i], both(n.to_code));
+                const float2 q = code_quotient<OUT>(t[k].p[i], n);
                 c[i] = ocp_encode2<OUT>(q.x, q.y);
             }
             uint8_t* o = a.codes + at;

@@ -8,8 +8,9 @@ Tolerances (u = 2^-24, one fp32 rounding):
   R = (cols / 32 + 34) / 2 u + 2 u, and y = t r within R + 2 u, plus the
   type's rounding.
 - 8-bit scales r T / qmax: R + 4 u.  A code is the nearest value of a quotient
-  t (qmax / T) that has three roundings, so its distance from the exact quotient is
-  half a step plus 4 u |q|.
+  t qmax / T whose t, T and division are rounded, so its distance from the exact
+  quotient is half a step plus 4 u |q|.  For bf16 tensors t is exact and the codes are the
+  correctly rounded ones, value for value.
 - NVFP4 codes are compared like those of fp32 values (scales 2^-20, codes 2^-17);
   t itself is a rounded product (u of it): 2^-19 and 2^-16 (|q| <= 9).
   MXFP4 codes of y: y within R + 2 u, so a border moves by 8 (R + 2 u), and a block's
@@ -67,14 +68,24 @@ def half_step(q, fmt):
     return np.ldexp(0.5, e - 1 - bits)
 
 
-def check_codes8(codes, scales, t, r, cols, fmt):
+def check_codes8(codes, scales, t, r, cols, fmt, exact=False):
     T = np.abs(t).max(1)
     level = np.maximum(T, 2.0 ** -110)
     want = np.where(T > 0, r * level / R.QMAX[fmt], 1.0)
     s = scales.double().cpu().numpy()
     assert np.all(np.abs(s - want) <= want * (tol_r(cols) + 4 * U))
-    q = t * (R.QMAX[fmt] / level)[:, None]
+    q = t * R.QMAX[fmt] / level[:, None]   # one rounding of exact products: borders stay borders
     got = code_values(codes, fmt)
+    if exact:
+        bits = {E4M3: (3, -6), E5M2: (2, -14)}
+        if fmt == INT8:
+            want_q = np.rint(q)
+        else:
+            mant, low = bits[fmt]
+            _, e = np.frexp(np.maximum(np.abs(q), 2.0 ** low))
+            s = np.ldexp(1.0, e - 1 - mant)
+            want_q = np.rint(q / s) * s
+        assert np.array_equal(got, want_q)
     # at the edge above a power of two the step doubles: take the wider one
     step = np.maximum(half_step(q, fmt), half_step(q * (1 + 8 * U), fmt))
     assert np.all(np.abs(got - q) <= step + 4 * U * np.abs(q))
@@ -173,7 +184,7 @@ def test_eight_bits(nq, bf16, shape):
                 assert np.array_equal(s.double().cpu().numpy(), h)
             t, r = R.rmsnorm(h, w.double().cpu().numpy(), EPS)
             check_y(y, t, r, cols)
-            check_codes8(codes, scales, t, r, cols, fmt)
+            check_codes8(codes, scales, t, r, cols, fmt, exact=bf16)
 
 
 @pytest.mark.parametrize("fmt", [R.MX, R.NV])
