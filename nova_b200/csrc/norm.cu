@@ -931,7 +931,6 @@ nq_status_t launch_grad(const GradArgs& a, float* dw, const DeviceInfo& di, cuda
         // the weight gradient's sum, does not depend on dx)
         const size_t row = static_cast<size_t>(a.cols) * sizeof(In) * (a.dsum ? 3 : 2);
         stages = static_cast<int>(std::max<size_t>(2, std::min<size_t>(4, 60 * 1024 / row)));
-        if (stages * row > kGradSmem) stages = 1;
         smem = stages * (row + 8);
         static std::mutex mu;
         static std::atomic<uint64_t> attr_set{0};

@@ -211,7 +211,9 @@ def test_dequantize_every_scale_byte(nq):
         scales[R.scale_index(1, 256 * n, fmt)] = np.arange(256, dtype=np.uint8)[None]
         out = dequantize(nq, torch.from_numpy(codes).cuda(), torch.from_numpy(scales).cuda(), None, 1, 256 * n, fmt, False)
         want = R.unpack_codes(codes, 1, 256 * n) * np.repeat(ref(np.arange(256)), n)[None]
-        assert np.array_equal(out.double().cpu().numpy(), want.astype(np.float32).astype(np.float64), equal_nan=True)
+        with np.errstate(over="ignore"):   # 6 * 2^127 is an infinity in fp32
+            want = want.astype(np.float32).astype(np.float64)
+        assert np.array_equal(out.double().cpu().numpy(), want, equal_nan=True)
 
 
 # ---- the product ---------------------------------------------------------------------
