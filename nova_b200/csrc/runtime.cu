@@ -71,6 +71,16 @@ nq_status_t current_device(DeviceInfo* out) {
     return NQ_SUCCESS;
 }
 
+namespace {
+// Lets this thread make calls that a stream capture in progress would forbid
+// (creating the pool allocates nothing on the captured stream).
+struct RelaxedCapture {
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+    ~RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+};
+}  // namespace
+
 nq_status_t scratch_alloc(void** p, size_t bytes, cudaStream_t s) {
     int dev = -1;
     NQ_CHECK_CUDA(cudaGetDevice(&dev), "cudaGetDevice");
@@ -80,6 +90,7 @@ nq_status_t scratch_alloc(void** p, size_t bytes, cudaStream_t s) {
         std::lock_guard<std::mutex> lk(g_mu);
         pool = g_pool[dev].load(std::memory_order_relaxed);
         if (!pool) {
+            const RelaxedCapture relaxed;  // the first call may be inside a capture
             cudaMemPoolProps props = {};
             props.allocType = cudaMemAllocationTypePinned;
             props.location.type = cudaMemLocationTypeDevice;

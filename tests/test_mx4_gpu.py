@@ -510,3 +510,50 @@ def test_two_threads_at_once(nq):
         t.join(120)
     torch.cuda.synchronize()
     assert not failed and nq.device_error_flags() == 0
+
+
+FIRST_CALL = """
+import ctypes as C, sys, torch
+import nova_b200.capi as nq
+x, w = torch.randn(600, 4096, device="cuda").bfloat16(), torch.randn(4096, device="cuda").bfloat16()
+u8 = lambda n: torch.zeros(n, dtype=torch.uint8, device="cuda")
+codes, scales, g = u8(600 * nq.mx4_row_bytes(16384)), u8(nq.mx4_scale_bytes(600, 16384, 1)), torch.ones(600, device="cuda")
+out, dx, dw = torch.empty(600, 600, device="cuda"), torch.empty_like(x), torch.full((4096,), 7.0, device="cuda")
+norm = nq.make_rmsnorm_desc(600, 4096, nq.BF16, nq.BF16, 1e-5)
+gemm = nq.make_mx4_desc(4, 256, 16384, 1, nq.F32, 1.0)
+p = lambda t: t.data_ptr()
+
+def go():
+    s = torch.cuda.current_stream().cuda_stream
+    if sys.argv[1] == "norm":
+        nq.rmsnorm_quantize_mx4(C.byref(norm), p(x), 0, p(w), 0, p(dx), p(codes), p(scales), p(g), 1, s)
+    elif sys.argv[1] == "backward":
+        nq.rmsnorm_backward(C.byref(norm), p(x), p(w), p(x), 0, p(dx), p(dw), s)
+    elif sys.argv[1] == "quantize":
+        nq.quantize_rows_mx4(p(x), nq.BF16, 0, p(codes), p(scales), p(g), 600, 4096, 1, s)
+    else:
+        nq.gemm_mx4(C.byref(gemm), p(codes), p(scales), p(codes), p(scales), p(out), s)
+
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    go()
+graph.replay()
+torch.cuda.synchronize()
+got = [t.clone() for t in (codes, scales, g, out[:4], dx, dw)]
+go()
+torch.cuda.synchronize()
+assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(got, (codes, scales, g, out[:4], dx, dw)))
+assert nq.device_error_flags() == 0
+print("captured")
+"""
+
+
+@pytest.mark.parametrize("what", ["norm", "backward", "quantize", "product"])
+def test_first_call_of_a_process_captured(nq, what):
+    """The library's first call may already be inside a capture (its pool is then created there)."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", FIRST_CALL, what], cwd=root, capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
