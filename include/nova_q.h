@@ -431,10 +431,11 @@ nq_status_t nq_gemm_mx4(const nq_gemm_mx4_desc_t* desc, const uint8_t* a_codes, 
  *           must be dense).  Only with a residual;
  *   y       y rounded to the tensors' type, dense, or NULL;
  *   codes   the quantized y, or NULL (then scales is NULL too).
- * 8-bit output, as nq_quantize_rows defines it (a row's factor r cancels in the
- * codes): T = max |t|, scales[r] = r T / qmax (1.0 for T = 0), code =
- * encode(t qmax / T), T at least 2^-110, the quotient rounded once.  A row that holds an infinity or
- * NaN has a NaN scale.  4-bit output: NQ_MXFP4 of y; NQ_NVFP4 codes and block
+ * 8-bit output with a scale a row, as nq_quantize_rows gives it (a row's factor r
+ * cancels in the codes): T = max |t|, scales[r] = r T / qmax (1.0 for T = 0),
+ * code = encode(t qmax / T), T at least 2^-110; t, t qmax and the quotient are
+ * rounded to fp32 once each.  A row that holds an infinity or NaN, or whose t
+ * leaves fp32's range, has a NaN scale.  4-bit output: NQ_MXFP4 of y; NQ_NVFP4 codes and block
  * scales of t, row scale r A / 2688. */
 typedef struct {
     int rows, cols;

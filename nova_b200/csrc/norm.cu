@@ -128,20 +128,22 @@ __device__ __forceinline__ void block_sum_max(float& s, uint32_t& m, int parity)
 
 // What a row's reduction gives the encoder.
 struct RowNorm {
-    float r;        // 1 / rms (where it is needed: y, MXFP4)
-    float tn, inv;  // 8 bits: T / 512 and its reciprocal
-    NvRow nv;       // NVFP4
+    float r;             // 1 / rms (where it is needed: y, MXFP4)
+    float mul, tn, inv;  // 8 bits: qmax p and T p for a power of two p, and the reciprocal of T p
+    NvRow nv;            // NVFP4
 };
 __device__ __forceinline__ float row_r(float sumsq, float inv_cols, float eps) {
     return rsqrtf(__fmaf_rn(sumsq, inv_cols, eps));
 }
-// The quotient t qmax / T of an 8-bit code, correctly rounded: a product with the
-// reciprocal, its remainder, one correction.  (Quotients of bf16 products are ratios of
-// small integers and fall on rounding borders; the product alone puts them to
-// either side.)
-template <int F>
+// The quotient t qmax / T of an 8-bit code: numerator rounded (exact for bf16 tensors), then a
+// product with the reciprocal, its remainder, one correction: the quotient correctly
+// rounded.  (Quotients of bf16 products are ratios of small integers and fall on
+// rounding borders; the product alone puts them to either side.)
+// Numerator and denominator carry a power of two by the row's T: 2^-16 from 1 on, so that
+// |t| qmax 2^-16 <= 0.875 T whatever the format, and 2^32 below, so that neither the numerator of a code
+// that is not zero nor a remainder is subnormal (T >= 2^-110).
 __device__ __forceinline__ float2 code_quotient(float2 t, const RowNorm& n) {
-    const float2 num = mul2(t, both(FmtTraits<F>::qmax / 512.0f));  // (scaled so that nothing overflows)
+    const float2 num = mul2(t, both(n.mul));
     const float2 q = mul2(num, both(n.inv));
     return fma2(fma2(q, both(-n.tn), num), both(n.inv), q);
 }
@@ -154,7 +156,9 @@ __device__ __forceinline__ RowNorm row_norm(const NormArgs& a, int row, float su
     if (OUT <= kOutINT8) {
         constexpr float qmax = FmtTraits<OUT <= kOutINT8 ? OUT : 0>::qmax;
         const float T = fmaxf(__uint_as_float(tmax), 0x1p-110f);
-        n.tn = T * 0x1p-9f;
+        const float p = T < 1.0f ? 0x1p32f : 0x1p-16f;
+        n.mul = qmax * p;
+        n.tn = T * p;
         n.inv = __frcp_rn(n.tn);
         if (first)
             a.scales[row] = tmax >= kInfBits ? __uint_as_float(0x7FC00000u)
@@ -191,7 +195,7 @@ __device__ __forceinline__ void emit8(const NormArgs& a, int row, int v, const M
         uint32_t c[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const float2 q = code_quotient<F>(t.p[i], n);
+            const float2 q = code_quotient(t.p[i], n);
             c[i] = ocp_encode2<F>(q.x, q.y);
         }
         store_codes8<VEC>(a.codes + static_cast<size_t>(row) * a.cols, v, a.cols, make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16)), buf);
@@ -415,7 +419,7 @@ __global__ void __launch_bounds__(SMALL ? 320 : 1024, SMALL ? 4 : 1) k_norm_cut(
             uint32_t c[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float2 q = code_quotient<OUT>(t[k].p[i], n);
+                const float2 q = code_quotient(t[k].p[i], n);
                 c[i] = ocp_encode2<OUT>(q.x, q.y);
             }
             uint8_t* o = a.codes + at;

@@ -436,3 +436,28 @@ def test_dense_unaligned_base(nq, bf16):
         t, r = R.rmsnorm(h, w.double().cpu().numpy(), EPS)
         check_y(y, t, r, cols)
         check_codes8(codes, scales, t, r, cols, E4M3)
+
+
+def product32(h, w):
+    """t = h w as fp32 rounds it (a double holds the exact product of two fp32 values)."""
+    return (h * w).astype(np.float32).astype(np.float64)
+
+
+@pytest.mark.parametrize("bf16", [True, False])
+@pytest.mark.parametrize("shape", [(9, 96), (9, 1024), (9, 1003), (700, 2048), (3, 40000), (2, 33001)])
+@pytest.mark.parametrize("scale", [1e-36, 1e-30, 1e30, 3e37])
+def test_eight_bits_of_extreme_weights(nq, bf16, shape, scale):
+    """Finite rows of any magnitude of h w have the codes of t qmax / T: nothing on the way leaves fp32's range."""
+    import torch
+    rows, cols = shape
+    x, w = rand(rows, cols, 1, bf16).clamp(-4, 4), (rand(1, cols, 2, False).view(-1).clamp(-2, 2) * scale)
+    w = w.to(x.dtype)
+    if scale < 1:   # a row of both ends
+        x[:, 0], w[0] = 0.0, 1.0
+        x[1, 0] = 1.0
+    h, w64 = reference_h(x, None), w.double().cpu().numpy()
+    t, r = product32(h, w64), R.rmsnorm(h, 1.0, EPS)[1]
+    assert np.isfinite(t).all()
+    for fmt in (E4M3, E5M2, INT8):
+        _, codes, _, scales = run(nq, x, None, w, fmt, want_y=False)
+        check_codes8(codes, scales, t, r, cols, fmt, exact=bf16)
