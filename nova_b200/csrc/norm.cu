@@ -147,6 +147,15 @@ __device__ __forceinline__ float2 code_quotient(float2 t, const RowNorm& n) {
     const float2 q = mul2(num, both(n.inv));
     return fma2(fma2(q, both(-n.tn), num), both(n.inv), q);
 }
+// Row scales of the 8-bit formats and of NVFP4 (tmax: magnitude bits of the largest t).
+template <int F>
+__device__ __forceinline__ float row_scale8(float r, uint32_t tmax) {
+    if (tmax >= kInfBits) return __uint_as_float(0x7FC00000u);
+    return tmax == 0u ? 1.0f : __fdiv_rn(__fmul_rn(r, fmaxf(__uint_as_float(tmax), 0x1p-110f)), FmtTraits<F>::qmax);
+}
+__device__ __forceinline__ float row_scale_nv(float r, uint32_t tmax, float level) {
+    return tmax == 0u ? 1.0f : __fmul_rn(r, nv_row_scale(tmax, level));
+}
 // `first`: this thread stores the row's scale (the only place, besides y and
 // MXFP4, where r and its divisions are needed).
 template <int OUT>
@@ -160,15 +169,110 @@ __device__ __forceinline__ RowNorm row_norm(const NormArgs& a, int row, float su
         n.mul = qmax * p;
         n.tn = T * p;
         n.inv = __frcp_rn(n.tn);
-        if (first)
-            a.scales[row] = tmax >= kInfBits ? __uint_as_float(0x7FC00000u)
-                                             : (tmax == 0u ? 1.0f : __fdiv_rn(__fmul_rn(row_r(sumsq, a.inv_cols, a.eps), T), qmax));
+        if (first) a.scales[row] = row_scale8<OUT <= kOutINT8 ? OUT : 0>(row_r(sumsq, a.inv_cols, a.eps), tmax);
     } else if (OUT == kOutNV) {
         n.nv = nv_row(tmax);
-        if (first)
-            a.scales[row] = tmax == 0u ? 1.0f : __fmul_rn(row_r(sumsq, a.inv_cols, a.eps), nv_row_scale(tmax, n.nv.level));
+        if (first) a.scales[row] = row_scale_nv(row_r(sumsq, a.inv_cols, a.eps), tmax, n.nv.level);
     }
     return n;
+}
+
+// Rows whose sum(h^2) is out of fp32's range (a finite |h| from 1.8e19 on may do that): what
+// depends on r -- the row scale, y, MXFP4 codes -- once more, with the sum of (h 2^-80)^2, which
+// 2^30 finite columns keep in range.  The other codes are right as they are.  A block or warp
+// that met such a row does this for all its rows when it is through with them: inside the loop over
+// rows it cost the kernels up to 17%.  (A sum within a factor of two of the border is taken here
+// too: the same r but for rounding.)  h comes from sum where that is stored, which may
+// have taken the place of an input.
+template <class In, int OUT, bool WARP>
+__device__ __forceinline__ void redo_far_rows_of(const NormArgs& a, long long first, long long step, int t0, int width) {
+    constexpr float far = 0x1p-80f;
+    auto value = [](const In* p, int c) {
+        if constexpr (sizeof(In) == 4) return p[c];
+        else return bf16_bits_to_f32(p[c]);
+    };
+    auto weight = [&](int c) {
+        return (a.w_kind & 1) ? bf16_bits_to_f32(static_cast<const uint16_t*>(a.w)[c]) : static_cast<const float*>(a.w)[c];
+    };
+    if (WARP) __syncwarp();
+    else __syncthreads();
+    int parity = 0;
+    for (long long rl = first; rl < a.rows; rl += step, parity ^= 1) {
+        const int row = static_cast<int>(rl);
+        const In* x = a.sum ? static_cast<const In*>(a.sum) + static_cast<size_t>(row) * a.cols
+                            : static_cast<const In*>(a.x) + row * a.x_stride;
+        const In* res = a.res && !a.sum ? static_cast<const In*>(a.res) + row * a.res_stride : nullptr;
+        auto load_h = [&](int c) {
+            float h = value(x, c);
+            if (res) h = __fadd_rn(h, value(res, c));
+            if (res && sizeof(In) == 2) h = bf16_bits_to_f32(f32x2_to_bf16x2(h, 0.0f) & 0xFFFFu);
+            return h;
+        };
+        float s = 0.0f;
+        uint32_t tm = 0;
+#pragma unroll 1
+        for (int c = t0; c < a.cols; c += width) {
+            const float h = load_h(c), hs = __fmul_rn(h, far);
+            s = __fmaf_rn(hs, hs, s);
+            tm = max(tm, __float_as_uint(__fmul_rn(h, weight(c))) & 0x7FFFFFFFu);
+        }
+        if (WARP) {
+#pragma unroll
+            for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+            tm = __reduce_max_sync(0xffffffffu, tm);
+        } else {
+            block_sum_max(s, tm, parity);
+        }
+        if (s < 0.5f * FLT_MAX * far * far) continue;
+        const float r = far * rsqrtf(__fmaf_rn(s, a.inv_cols, a.eps * far * far));
+        if (t0 == 0) {
+            if (OUT <= kOutINT8) a.scales[row] = row_scale8<OUT <= kOutINT8 ? OUT : 0>(r, tm);
+            if (OUT == kOutNV) a.scales[row] = row_scale_nv(r, tm, nv_row(tm).level);
+        }
+        if (a.y) {
+            In* y = static_cast<In*>(a.y) + static_cast<size_t>(row) * a.cols;
+#pragma unroll 1
+            for (int c = t0; c < a.cols; c += width) {
+                const float v = __fmul_rn(__fmul_rn(load_h(c), weight(c)), r);
+                if constexpr (sizeof(In) == 4) y[c] = v;
+                else y[c] = static_cast<uint16_t>(f32x2_to_bf16x2(v, 0.0f));
+            }
+        }
+        if (OUT == kOutMX) {
+            const Mx4Row to = mx4_row(a.codes, a.bscales, row, a.cols, mx4_words(a.cols, 32));
+#pragma unroll 1
+            for (int b = t0; 32 * b < a.cols; b += width) {
+                auto y8 = [&](int q) {  // columns [32 b + 8 q, + 8)
+                    float e[8];
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const int c = 32 * b + 8 * q + k;
+                        e[k] = c < a.cols ? __fmul_rn(__fmul_rn(load_h(c), weight(c)), r) : 0.0f;
+                    }
+                    return F8{{{e[0], e[1]}, {e[2], e[3]}, {e[4], e[5]}, {e[6], e[7]}}};
+                };
+                uint32_t m = 0;
+#pragma unroll 1
+                for (int q = 0; q < 4; ++q) m = max(m, amax_bits8(y8(q)));
+                const Mx4Block k = mx4_block<kMXFP4, false>(m, NvRow{});
+#pragma unroll 1
+                for (int q = 0; q < 4; ++q) to.codes[4 * b + q] = mx4_codes8<kMXFP4, false>(y8(q), k);
+                to.scales[static_cast<size_t>(b / 4) * 512 + b % 4] = static_cast<uint8_t>(k.byte);
+            }
+        }
+    }
+}
+
+// Called or inline, as the loop before it compiles better: 65536 x 203 bf16 to E4M3 50 us called, 57
+// inline; 65536 x 1024 bf16 to MXFP4 84 called, 73 inline.
+template <class In, int OUT, bool WARP>
+__device__ __noinline__ void redo_far_call(const NormArgs& a, long long first, long long step, int t0, int width) {
+    redo_far_rows_of<In, OUT, WARP>(a, first, step, t0, width);
+}
+template <class In, int OUT, bool WARP>
+__device__ __forceinline__ void redo_far_rows(const NormArgs& a, long long first, long long step, int t0, int width) {
+    if (OUT == kOutMX) redo_far_rows_of<In, OUT, WARP>(a, first, step, t0, width);
+    else redo_far_call<In, OUT, WARP>(a, first, step, t0, width);
 }
 
 // Encodes and stores this thread's 8 columns of a row (every lane takes part).
@@ -205,7 +309,7 @@ __device__ __forceinline__ void emit8(const NormArgs& a, int row, int v, const M
 // One block per row in two passes: the reduction, then the encoding of the row
 // read again (from sum where it is stored).  For rows too wide for k_norm_rows.
 template <class In, int OUT, bool VEC>
-__global__ void __launch_bounds__(256) k_norm_two_pass(const NormArgs a) {
+__global__ void __launch_bounds__(256) k_norm_two_pass(const __grid_constant__ NormArgs a) {
     pdl_launch_dependents();
     pdl_wait();
     uint8_t* buf = warp_buf<VEC>();
@@ -216,6 +320,7 @@ __global__ void __launch_bounds__(256) k_norm_two_pass(const NormArgs a) {
     const int nstep = four ? words * Mx4Traits<F>::word_lanes : nvec;
     const int lane = lane_of();
     int parity = 0;
+    bool far = false;  // some row's sum(h^2) left fp32's range
     for (long long rl = blockIdx.x; rl < a.rows; rl += gridDim.x, parity ^= 1) {
         const int row = static_cast<int>(rl);
         const In* x = static_cast<const In*>(a.x) + row * a.x_stride;
@@ -235,6 +340,7 @@ __global__ void __launch_bounds__(256) k_norm_two_pass(const NormArgs a) {
         float ss = s2.x + s2.y;
         block_sum_max(ss, tm, parity);  // (its barrier also orders the unaligned rows' stores before the loads below)
         const Mx4Row to = four ? mx4_row(a.codes, a.bscales, row, a.cols, words) : Mx4Row{};
+        far |= !(ss <= FLT_MAX);
         const RowNorm n = row_norm<OUT>(a, row, ss, tm, threadIdx.x == 0);
         for (int v = threadIdx.x; v - lane < nstep; v += blockDim.x) {
             F8 t = unpack8<In>(sum ? load_vec<In, VEC>(sum, v, a.cols, buf) : load_h(v));
@@ -244,13 +350,14 @@ __global__ void __launch_bounds__(256) k_norm_two_pass(const NormArgs a) {
             emit8<In, OUT, VEC>(a, row, v, to, t, n, buf);
         }
     }
+    if (far) redo_far_rows<In, OUT, false>(a, blockIdx.x, gridDim.x, threadIdx.x, blockDim.x);
 }
 
 // Rows held in registers: a row is read once, 8 columns a vector and NV vectors
 // a thread, by one warp (WARP, 8 rows a block) or one block; the block's
 // threads are as many as the row needs.
 template <class In, int OUT, bool VEC, int NV, bool WARP>
-__global__ void __launch_bounds__(WARP ? 256 : 1024) k_norm_rows(const NormArgs a) {
+__global__ void __launch_bounds__(WARP ? 256 : 1024) k_norm_rows(const __grid_constant__ NormArgs a) {
     pdl_launch_dependents();
     uint8_t* buf = warp_buf<VEC>();
     constexpr int F = OUT == kOutNV ? kNVFP4 : kMXFP4;
@@ -267,6 +374,7 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) k_norm_rows(const NormArgs 
     }
     pdl_wait();
     int parity = 0;
+    bool far = false;  // some row's sum(h^2) left fp32's range
     for (long long rl = static_cast<long long>(blockIdx.x) * per + (WARP ? threadIdx.x >> 5 : 0); rl < a.rows;
          rl += static_cast<long long>(gridDim.x) * per, parity ^= 1) {
         const int row = static_cast<int>(rl);
@@ -299,6 +407,7 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) k_norm_rows(const NormArgs 
             block_sum_max(ss, tm, parity);
         }
         const Mx4Row to = four ? mx4_row(a.codes, a.bscales, row, a.cols, words) : Mx4Row{};
+        far |= !(ss <= FLT_MAX);
         const RowNorm n = row_norm<OUT>(a, row, ss, tm, t0 == 0);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
@@ -310,6 +419,9 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) k_norm_rows(const NormArgs 
             emit8<In, OUT, VEC>(a, row, v, to, t, n, buf);
         }
     }
+    if (far)
+        redo_far_rows<In, OUT, WARP>(a, static_cast<long long>(blockIdx.x) * per + (WARP ? threadIdx.x >> 5 : 0),
+                                     static_cast<long long>(gridDim.x) * per, t0, width);
 }
 
 // Dense rows of a width that is not a multiple of 8, 8-bit output: all tensors are
@@ -374,11 +486,12 @@ __device__ __forceinline__ F8 load_weight_cut(const void* w, int w_kind, int c0,
 }
 
 template <class In, int OUT, int NV, bool SMALL>
-__global__ void __launch_bounds__(SMALL ? 320 : 1024, SMALL ? 4 : 1) k_norm_cut(const NormArgs a) {
+__global__ void __launch_bounds__(SMALL ? 320 : 1024, SMALL ? 4 : 1) k_norm_cut(const __grid_constant__ NormArgs a) {
     pdl_launch_dependents();
     pdl_wait();
     const int width = blockDim.x, t0 = threadIdx.x;
     int parity = 0;
+    bool far = false;  // some row's sum(h^2) left fp32's range
     for (long long rl = blockIdx.x; rl < a.rows; rl += gridDim.x, parity ^= 1) {
         const int row = static_cast<int>(rl);
         const int s = static_cast<int>((a.shift0 + rl * a.cols) & 7);
@@ -406,6 +519,7 @@ __global__ void __launch_bounds__(SMALL ? 320 : 1024, SMALL ? 4 : 1) k_norm_cut(
             t[k] = row_terms(unpack8<In>(h[k]), load_weight_cut(a.w, a.w_kind, 8 * (t0 + k * width) - s, a.cols), s2, tm);
         float ss = s2.x + s2.y;
         block_sum_max(ss, tm, parity);
+        far |= !(ss <= FLT_MAX);
         const RowNorm n = row_norm<OUT>(a, row, ss, tm, t0 == 0);
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
@@ -432,12 +546,15 @@ __global__ void __launch_bounds__(SMALL ? 320 : 1024, SMALL ? 4 : 1) k_norm_cut(
             }
         }
     }
+    if (far) redo_far_rows<In, OUT, false>(a, blockIdx.x, gridDim.x, t0, width);
 }
 
 // Many aligned rows: they come through a ring in shared memory by 1-D bulk
 // copies, so that the next rows stream in while one is reduced and encoded.
+// (Registers for as many blocks as the ring leaves room for: without the bound 16384 x 4096 bf16
+// to NVFP4 takes 133 us for 116.)
 template <class In, int OUT, int NV>
-__global__ void __launch_bounds__(512) k_norm_ring(const NormArgs a, int stages, uint32_t* err) {
+__global__ void __launch_bounds__(sizeof(In) == 2 ? 256 : 512, sizeof(In) == 2 ? (NV == 2 ? 3 : 2) : 0) k_norm_ring(const __grid_constant__ NormArgs a, int stages, uint32_t* err) {
     extern __shared__ __align__(128) uint8_t n_smem[];
     pdl_launch_dependents();
     constexpr int F = OUT == kOutNV ? kNVFP4 : kMXFP4;
@@ -467,6 +584,7 @@ __global__ void __launch_bounds__(512) k_norm_ring(const NormArgs a, int stages,
     if (t0 == 0)
         for (int i = 0; i < stages; ++i) issue(i);
     int st = 0, parity = 0;
+    bool far = false;
     uint32_t phase = 0;
     bool ok = true;  // after a wait that ran out (error bit set) a thread waits and issues no more
     for (long long i = 0; blockIdx.x + i * gridDim.x < a.rows; ++i, parity ^= 1) {
@@ -493,6 +611,7 @@ __global__ void __launch_bounds__(512) k_norm_ring(const NormArgs a, int stages,
         block_sum_max(ss, tm, parity);
         if (t0 == 0 && ok) issue(i + stages);  // every thread has read the stage
         const Mx4Row to = four ? mx4_row(a.codes, a.bscales, row, a.cols, words) : Mx4Row{};
+        far |= !(ss <= FLT_MAX);
         const RowNorm n = row_norm<OUT>(a, row, ss, tm, t0 == 0);
 #pragma unroll
         for (int k = 0; k < NV; ++k) emit8<In, OUT, true>(a, row, t0 + k * width, to, t[k], n, nullptr);
@@ -501,6 +620,7 @@ __global__ void __launch_bounds__(512) k_norm_ring(const NormArgs a, int stages,
     if (!ok && t0 == 0)  // copies still in flight land before the block ends
         for (long long k = max(0ll, last - stages + 1); k <= last; ++k)
             mbar_wait(&full[k % stages], static_cast<uint32_t>(k / stages) & 1u, nullptr);
+    if (far) redo_far_rows<In, OUT, false>(a, blockIdx.x, gridDim.x, t0, width);
 }
 
 // ---- gradient ---------------------------------------------------------------------

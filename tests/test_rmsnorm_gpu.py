@@ -461,3 +461,50 @@ def test_eight_bits_of_extreme_weights(nq, bf16, shape, scale):
     for fmt in (E4M3, E5M2, INT8):
         _, codes, _, scales = run(nq, x, None, w, fmt, want_y=False)
         check_codes8(codes, scales, t, r, cols, fmt, exact=bf16)
+
+
+def far_rows(x, scale):
+    """Rows of finite values whose squares leave fp32's range: all of them, and one column alone."""
+    x = x.clamp(-4, 4) * scale
+    x[1] /= scale
+    x[1, 3] = scale
+    return x
+
+
+# widths and heights of every forward kernel: a warp a row, a block a row, many rows, odd widths, wide ones
+FAR_SHAPES = [(9, 96), (9, 77), (9, 1024), (9, 1003), (700, 2048), (3, 40000), (3, 33001)]
+
+
+@pytest.mark.parametrize("bf16", [True, False])
+@pytest.mark.parametrize("shape", FAR_SHAPES)
+@pytest.mark.parametrize("scale", [1e20, 1e30, 5e37])
+def test_rows_whose_squares_overflow(nq, bf16, shape, scale):
+    """sum(h^2) beyond fp32: r, y and the scales are those of the formula, for any finite row.
+
+    Squares of h 2^-80: the same roundings as in range; a subnormal r (rms above 2^126) or y is off by 2^-150 more
+    (2^-134 for a bf16 y)."""
+    import torch
+    rows, cols = shape
+    x = far_rows(rand(rows, cols, 1, bf16), scale)
+    res = rand(rows, cols, 2, bf16)
+    w = (rand(1, cols, 3, False).view(-1).clamp(-0.4, 0.4) + 1.0).to(x.dtype)
+    w64 = w.double().cpu().numpy()
+    for r_, with_sum in ((None, False), (res, False), (res, True)):
+        s = torch.empty_like(x) if with_sum else None
+        h = reference_h(x, r_)
+        t, r = product32(h, w64), R.rmsnorm(h, 1.0, EPS)[1]
+        assert np.isfinite(t).all()
+        for fmt in (E4M3, E5M2, INT8):
+            y, codes, _, scales = run(nq, x, r_, w, fmt, sum=s)
+            check_codes8(codes, scales, t, r, cols, fmt, exact=bf16)
+            assert s is None or np.array_equal(s.double().cpu().numpy(), h)
+        ref = t * r[:, None]
+        half, low = (2.0 ** -8, 2.0 ** -134) if bf16 else (0.0, 2.0 ** -150)
+        assert np.all(np.abs(y.double().cpu().numpy() - ref) <= np.abs(ref) * (tol_r(cols) + 2 * U + half) + 2 * low)
+        for fmt in (R.MX, R.NV):
+            _, codes, bs, g = run(nq, x, r_, w, fmt, four=True, sum=s, want_y=False)
+            check_mx4(nq, (codes, bs, g), t, r, rows, cols, fmt)
+    for bad in (float("inf"), float("nan")):   # a row that is not finite beside them
+        x[2, 5] = bad
+        y, codes, _, scales = run(nq, x, None, w, E4M3)
+        assert torch.isnan(scales[2]) and torch.isfinite(scales[[0, 1]]).all() and torch.isnan(y[2, 5])
