@@ -177,6 +177,7 @@ __device__ __forceinline__ RowNorm row_norm(const NormArgs& a, int row, float su
     return n;
 }
 
+constexpr float kFar = 0x1p-80f;
 // Rows whose sum(h^2) is out of fp32's range (a finite |h| from 1.8e19 on may do that): what
 // depends on r -- the row scale, y, MXFP4 codes -- once more, with the sum of (h 2^-80)^2, which
 // 2^30 finite columns keep in range.  The other codes are right as they are.  A block or warp
@@ -186,7 +187,6 @@ __device__ __forceinline__ RowNorm row_norm(const NormArgs& a, int row, float su
 // have taken the place of an input.
 template <class In, int OUT, bool WARP>
 __device__ __forceinline__ void redo_far_rows_of(const NormArgs& a, long long first, long long step, int t0, int width) {
-    constexpr float far = 0x1p-80f;
     auto value = [](const In* p, int c) {
         if constexpr (sizeof(In) == 4) return p[c];
         else return bf16_bits_to_f32(p[c]);
@@ -212,7 +212,7 @@ __device__ __forceinline__ void redo_far_rows_of(const NormArgs& a, long long fi
         uint32_t tm = 0;
 #pragma unroll 1
         for (int c = t0; c < a.cols; c += width) {
-            const float h = load_h(c), hs = __fmul_rn(h, far);
+            const float h = load_h(c), hs = __fmul_rn(h, kFar);
             s = __fmaf_rn(hs, hs, s);
             tm = max(tm, __float_as_uint(__fmul_rn(h, weight(c))) & 0x7FFFFFFFu);
         }
@@ -223,8 +223,8 @@ __device__ __forceinline__ void redo_far_rows_of(const NormArgs& a, long long fi
         } else {
             block_sum_max(s, tm, parity);
         }
-        if (s < 0.5f * FLT_MAX * far * far) continue;
-        const float r = far * rsqrtf(__fmaf_rn(s, a.inv_cols, a.eps * far * far));
+        if (s < 0.5f * FLT_MAX * kFar * kFar) continue;
+        const float r = kFar * row_r(s, a.inv_cols, a.eps * kFar * kFar);
         if (t0 == 0) {
             if (OUT <= kOutINT8) a.scales[row] = row_scale8<OUT <= kOutINT8 ? OUT : 0>(r, tm);
             if (OUT == kOutNV) a.scales[row] = row_scale_nv(r, tm, nv_row(tm).level);
@@ -660,16 +660,34 @@ __device__ __forceinline__ void block_sum2(float& s, float& g, int parity) {
     }
 }
 
-// Row terms of the gradient: dx = dsum + r g - c h, c = r^2 mean(g n), n = h r
-// (the bounded form: |mean(g n)| <= max |g|).
+// Row terms of the gradient: dx = dsum + r (g - m n), n = h r, m = mean(g n).  |m| <= max |g|: in
+// range whatever r is (r^2, in the form r g - r^2 m h, leaves fp32 for rows of 1e18 or of 1e-19).
 struct RowGrad {
-    float r, c;
+    float r, m;
 };
 __device__ __forceinline__ RowGrad row_grad(const GradArgs& a, float sumsq, float sgh) {
     RowGrad q;
     q.r = row_r(sumsq, a.inv_cols, a.eps);
-    q.c = __fmul_rn(__fmul_rn(__fmul_rn(sgh, q.r), a.inv_cols), __fmul_rn(q.r, q.r));
+    q.m = __fmul_rn(__fmul_rn(sgh, q.r), a.inv_cols);
     return q;
+}
+__device__ __forceinline__ bool row_grad_ok(float sumsq, float sgh) { return sumsq <= FLT_MAX && fabsf(sgh) <= FLT_MAX; }
+// The same where a sum is out of range, from those with h 2^-80 in the place of h (sumsq: sum(h^2) itself).
+__device__ __forceinline__ RowGrad row_grad_far(const GradArgs& a, float sumsq, float far_sumsq, float far_sgh) {
+    const float r = sumsq <= FLT_MAX ? row_r(sumsq, a.inv_cols, a.eps) / kFar : row_r(far_sumsq, a.inv_cols, a.eps * kFar * kFar);
+    RowGrad q;
+    q.r = r * kFar;
+    q.m = __fmul_rn(__fmul_rn(far_sgh, r), a.inv_cols);
+    return q;
+}
+// (sums of a vector for it)
+__device__ __forceinline__ void grad_far_terms(const F8& h, const F8& gw, float2& ss, float2& sg) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = mul2(h.p[i], both(kFar));
+        ss = fma2(f, f, ss);
+        sg = fma2(gw.p[i], f, sg);
+    }
 }
 // gw = g w; ss += h^2, sg += gw h.
 __device__ __forceinline__ F8 grad_terms(const F8& h, const F8& g, const F8& w, float2& ss, float2& sg) {
@@ -682,13 +700,13 @@ __device__ __forceinline__ F8 grad_terms(const F8& h, const F8& g, const F8& w, 
     }
     return gw;
 }
-// r gw - c h [+ d]
-__device__ __forceinline__ F8 grad_dx(const F8& h, const F8& gw, const RowGrad& q, bool has_d, const F8& d) {
+// r (gw - m n) [+ d]
+__device__ __forceinline__ F8 grad_dx(const F8& n, const F8& gw, const RowGrad& q, bool has_d, const F8& d) {
     F8 o;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        o.p[i] = has_d ? fma2(both(-q.c), h.p[i], d.p[i]) : mul2(both(-q.c), h.p[i]);
-        o.p[i] = fma2(both(q.r), gw.p[i], o.p[i]);
+        o.p[i] = fma2(both(-q.m), n.p[i], gw.p[i]);
+        o.p[i] = has_d ? fma2(both(q.r), o.p[i], d.p[i]) : mul2(both(q.r), o.p[i]);
     }
     return o;
 }
@@ -714,17 +732,34 @@ __global__ void __launch_bounds__(256) k_norm_grad_rows(const GradArgs a, float*
                              load_weight8(a.w, a.w_kind, v, a.cols), s2, g2);
         float ss = s2.x + s2.y, sg = g2.x + g2.y;
         block_sum2(ss, sg, parity);
-        const RowGrad q = row_grad(a, ss, sg);
+        RowGrad q = row_grad(a, ss, sg);
+        if (!row_grad_ok(ss, sg)) {
+            s2 = g2 = both(0.0f);
+            for (int v = threadIdx.x; v - lane < nvec; v += blockDim.x) {
+                F8 g = unpack8<In>(load_vec<In, VEC>(dyp, v, a.cols, buf));
+                const F8 w = load_weight8(a.w, a.w_kind, v, a.cols);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) g.p[i] = mul2(g.p[i], w.p[i]);
+                grad_far_terms(unpack8<In>(load_vec<In, VEC>(hp, v, a.cols, buf)), g, s2, g2);
+            }
+            float fs = s2.x + s2.y, fg = g2.x + g2.y;
+            __syncthreads();  // the buffers of block_sum2 are free again
+            block_sum2(fs, fg, parity);
+            q = row_grad_far(a, ss, fs, fg);
+        }
         if (threadIdx.x == 0) rs[row] = q.r;
         if (!a.dx) continue;
         for (int v = threadIdx.x; v - lane < nvec; v += blockDim.x) {
-            const F8 h = unpack8<In>(load_vec<In, VEC>(hp, v, a.cols, buf));
+            F8 n = unpack8<In>(load_vec<In, VEC>(hp, v, a.cols, buf));
             const F8 w = load_weight8(a.w, a.w_kind, v, a.cols);
             F8 g = unpack8<In>(load_vec<In, VEC>(dyp, v, a.cols, buf)), d{};
             if (a.dsum) d = unpack8<In>(load_vec<In, VEC>(static_cast<const In*>(a.dsum) + at, v, a.cols, buf));
 #pragma unroll
-            for (int i = 0; i < 4; ++i) g.p[i] = mul2(g.p[i], w.p[i]);
-            store_vec<In, VEC>(static_cast<In*>(a.dx) + at, v, a.cols, pack8<In>(grad_dx(h, g, q, a.dsum, d)), buf);
+            for (int i = 0; i < 4; ++i) {
+                n.p[i] = mul2(n.p[i], both(q.r));
+                g.p[i] = mul2(g.p[i], w.p[i]);
+            }
+            store_vec<In, VEC>(static_cast<In*>(a.dx) + at, v, a.cols, pack8<In>(grad_dx(n, g, q, a.dsum, d)), buf);
         }
     }
 }
@@ -739,27 +774,53 @@ struct GradRow {
 template <class In, bool VEC, int NV, class Next>
 __device__ __forceinline__ void grad_row(const GradArgs& a, const GradRow<In, NV>& r, size_t at, int t0, int width, int parity,
                                          F8 (&acc)[NV], uint8_t* buf, Next next) {
+    // Of four vectors the products are formed again where they are needed: kept beside the branch
+    // below, they spill (4096 x 16384 bf16: 167 us for 160).
+    constexpr bool KEEP = NV < 4;
     float2 s2 = both(0.0f), g2 = both(0.0f);
-    F8 h[NV], gw[NV];
+    F8 gw[KEEP ? NV : 1];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        h[i] = unpack8<In>(r.h[i]);
-        gw[i] = grad_terms(h[i], unpack8<In>(r.g[i]), load_weight8(a.w, a.w_kind, t0 + i * width, a.cols), s2, g2);
+        const F8 p = grad_terms(unpack8<In>(r.h[i]), unpack8<In>(r.g[i]), load_weight8(a.w, a.w_kind, t0 + i * width, a.cols), s2, g2);
+        if constexpr (KEEP) gw[i] = p;
     }
+    auto product = [&](int i) {
+        if constexpr (KEEP) return gw[i];
+        int v = t0 + i * width;
+        asm volatile("" : "+r"(v));  // (a load of its own)
+        F8 p = unpack8<In>(r.g[i]);
+        const F8 w = load_weight8(a.w, a.w_kind, v, a.cols);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) p.p[j] = mul2(p.p[j], w.p[j]);
+        return p;
+    };
     float ss = s2.x + s2.y, sg = g2.x + g2.y;
     block_sum2(ss, sg, parity);
     next();
-    const RowGrad q = row_grad(a, ss, sg);
+    RowGrad q = row_grad(a, ss, sg);
+    if (!row_grad_ok(ss, sg)) {
+        s2 = g2 = both(0.0f);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) grad_far_terms(unpack8<In>(r.h[i]), product(i), s2, g2);
+        float fs = s2.x + s2.y, fg = g2.x + g2.y;
+        __syncthreads();  // the buffers of block_sum2 are free again
+        block_sum2(fs, fg, parity);
+        q = row_grad_far(a, ss, fs, fg);
+    }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
+        F8 n = unpack8<In>(r.h[i]);
         const F8 g = unpack8<In>(r.g[i]);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i].p[j] = fma2(mul2(h[i].p[j], both(q.r)), g.p[j], acc[i].p[j]);
+        for (int j = 0; j < 4; ++j) {
+            n.p[j] = mul2(n.p[j], both(q.r));
+            acc[i].p[j] = fma2(n.p[j], g.p[j], acc[i].p[j]);
+        }
         if (a.dx) {
             F8 d{};
             if (a.dsum) d = unpack8<In>(r.d[i]);
             store_vec<In, VEC>(static_cast<In*>(a.dx) + at, t0 + i * width, a.cols,
-                               pack8<In>(grad_dx(h[i], gw[i], q, a.dsum, d)), buf);
+                               pack8<In>(grad_dx(n, product(i), q, a.dsum, d)), buf);
         }
     }
 }

@@ -508,3 +508,51 @@ def test_rows_whose_squares_overflow(nq, bf16, shape, scale):
         x[2, 5] = bad
         y, codes, _, scales = run(nq, x, None, w, E4M3)
         assert torch.isnan(scales[2]) and torch.isfinite(scales[[0, 1]]).all() and torch.isnan(y[2, 5])
+
+
+def check_backward(nq, h, w, dy, ds, eps):
+    """Gradients against the formula's in 64 bits, within the roundings of the module's head."""
+    import torch
+    rows, cols = h.shape
+    bf16 = h.dtype == torch.bfloat16
+    dx, dw = torch.empty_like(h), torch.empty(cols, device="cuda")
+    d = nq.make_rmsnorm_desc(rows, cols, nq.BF16 if bf16 else nq.F32, nq.BF16 if bf16 else nq.F32, eps)
+    nq.rmsnorm_backward(C.byref(d), ptr(h), ptr(w), ptr(dy), ptr(ds), ptr(dx), ptr(dw), torch.cuda.current_stream().cuda_stream)
+    n64 = lambda t: None if t is None else t.double().cpu().numpy()
+    rx, rw = R.rmsnorm_backward(n64(h), n64(w), n64(dy), n64(ds), d.eps)
+    g, r = n64(dy) * n64(w), R.rmsnorm(n64(h), 1.0, d.eps)[1][:, None]
+    rp = (cols / 32 + 34) * U
+    tol = 2 * rp * (np.abs(r * g) + np.abs(n64(h)) * r ** 3 * np.abs(g * n64(h)).mean(1, keepdims=True))
+    tol = tol + (0 if ds is None else 2 * U * np.abs(n64(ds))) + np.abs(rx) * (2.0 ** -8 if bf16 else 2 * U)
+    tol = tol + (2.0 ** -133 if bf16 else 2.0 ** -147)   # subnormal results and products
+    assert np.all(np.abs(n64(dx) - rx) <= tol)
+    tol = np.abs(n64(dy) * n64(h) * r).sum(0) * (rows + 70 + 2 * tol_r(cols) / U) * U + rows * 2.0 ** -147
+    assert np.all(np.abs(n64(dw) - rw) <= tol)
+
+
+# widths and heights of every gradient kernel
+GRAD_SHAPES = [(9, 96), (9, 77), (200, 1024), (9, 1003), (5, 8192), (3, 16384), (3, 33001), (3, 40000)]
+
+
+@pytest.mark.parametrize("bf16", [True, False])
+@pytest.mark.parametrize("shape", GRAD_SHAPES)
+@pytest.mark.parametrize("scale,dscale,eps", [(1e18, 1e-6, EPS), (1e-19, 1e3, 1.1754944e-38), (0.0, 1e3, 1.1754944e-38)])
+def test_backward_of_far_scales(nq, bf16, shape, scale, dscale, eps):
+    """1 / rms^2 leaves fp32's range (or falls among its last bits) although no result does."""
+    rows, cols = shape
+    h, w = rand(rows, cols, 1, bf16, scale), rand(1, cols, 2, bf16).view(-1) + 1.0
+    dy, ds = rand(rows, cols, 3, bf16, dscale), rand(rows, cols, 4, bf16, dscale / max(scale, 1e-19))
+    for d in (None, ds):
+        check_backward(nq, h, w, dy, d, eps)
+
+
+@pytest.mark.parametrize("bf16", [True, False])
+@pytest.mark.parametrize("shape", GRAD_SHAPES)
+@pytest.mark.parametrize("scale,dscale", [(1e20, 1.0), (1e30, 1e-3), (1e34, 1.0), (1e10, 1e30)])
+def test_backward_of_rows_whose_sums_overflow(nq, bf16, shape, scale, dscale):
+    """sum(h^2), or sum(g h) alone, beyond fp32: the gradients are the formula's."""
+    rows, cols = shape
+    h, w = far_rows(rand(rows, cols, 1, bf16), scale), rand(1, cols, 2, bf16).view(-1) + 1.0
+    dy, ds = rand(rows, cols, 3, bf16, dscale), rand(rows, cols, 4, bf16, dscale / scale)
+    for d in (None, ds):
+        check_backward(nq, h, w, dy, d, EPS)
