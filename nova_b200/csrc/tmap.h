@@ -15,6 +15,29 @@ typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t,
                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
+// Binds the current device's context to a host thread that has none yet.  The runtime does so by itself,
+// the driver's cuTensorMapEncodeTiled does not (CUDA_ERROR_INVALID_CONTEXT): a product may be the
+// first thing that a thread does.
+inline nq_status_t bind_context() {
+    typedef CUresult (*CtxGetCurrentFn)(CUcontext*);
+    static std::atomic<CtxGetCurrentFn> cached{nullptr};
+    CtxGetCurrentFn f = cached.load(std::memory_order_acquire);
+    if (!f) {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        cudaError_t e = cudaGetDriverEntryPoint("cuCtxGetCurrent", &p, cudaEnableDefault, &q);
+        if (e != cudaSuccess || q != cudaDriverEntryPointSuccess || !p) return fail(NQ_ERROR_CUDA, "cuCtxGetCurrent entry point not found");
+        f = reinterpret_cast<CtxGetCurrentFn>(p);
+        cached.store(f, std::memory_order_release);
+    }
+    CUcontext ctx = nullptr;
+    if (f(&ctx) == CUDA_SUCCESS && ctx) return NQ_SUCCESS;
+    int dev = -1;
+    NQ_CHECK_CUDA(cudaGetDevice(&dev), "cudaGetDevice");
+    NQ_CHECK_CUDA(cudaSetDevice(dev), "cudaSetDevice");
+    return NQ_SUCCESS;
+}
+
 inline nq_status_t get_encode_fn(EncodeTiledFn* fn) {
     static std::atomic<EncodeTiledFn> cached{nullptr};
     static std::mutex mu;
@@ -33,7 +56,7 @@ inline nq_status_t get_encode_fn(EncodeTiledFn* fn) {
         }
     }
     *fn = f;
-    return NQ_SUCCESS;
+    return bind_context();
 }
 
 // 2-D uint8 tensor map: inner extent `inner`, `outer` rows of `ld` bytes,

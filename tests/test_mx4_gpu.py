@@ -557,3 +557,36 @@ def test_first_call_of_a_process_captured(nq, what):
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     r = subprocess.run([sys.executable, "-c", FIRST_CALL, what], cwd=root, capture_output=True, text=True, timeout=120)
     assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
+
+
+@pytest.mark.parametrize("m,n,k", [(300, 700, 512), (4, 4096, 28672), (8, 64, 64)])
+def test_first_call_of_a_thread(nq, m, n, k):
+    """A product as the first CUDA call that a host thread makes."""
+    import threading
+    import torch
+    a, _ = operand(m, k, R.NV, 1)
+    b, _ = operand(n, k, R.NV, 2)
+    i8 = lambda r, c: torch.randint(-127, 128, (r, c), dtype=torch.int8, device="cuda")
+    ia, ib = i8(m, k), i8(n, k)
+    ref = product(nq, a, b, m, n, k, R.NV, False)
+    outs = [torch.empty(m, n, device="cuda") for _ in range(2)]
+    gemm = nq.make_desc(m, n, k, nq.INT8, nq.INT8, nq.B_NK, nq.F32, 1.0)
+    eight = lambda o, s: nq.gemm(C.byref(gemm), ia.data_ptr(), ib.data_ptr(), o.data_ptr(), s)
+    s = torch.cuda.current_stream().cuda_stream
+    eight(outs[0], s)
+    out = torch.full_like(ref, 99.0)
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(call):
+        try:
+            call()
+        except Exception as e:
+            failed.append(repr(e))
+
+    for call in (lambda: product(nq, a, b, m, n, k, R.NV, False, out=out, stream=s), lambda: eight(outs[1], s)):
+        t = threading.Thread(target=work, args=(call,))
+        t.start()
+        t.join(60)
+    torch.cuda.synchronize()
+    assert not failed and torch.equal(out, ref) and torch.equal(*outs)
