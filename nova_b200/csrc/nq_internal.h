@@ -69,8 +69,9 @@ void scratch_free(void* p, cudaStream_t s);
 // Zero-initialised flag words owned by (current device, stream), at least
 // `count` of them, for kernels that clear every flag they raise before they
 // finish (so the next launch on the stream finds them zero without a memset).
-// While the stream is capturing a graph *p is nullptr: the caller then takes
-// flags from its scratch and clears them inside the graph.
+// While the stream is capturing a graph, and on streams behind the first 1024,
+// *p is nullptr: the caller then takes flags from its scratch and clears them
+// in the stream.
 nq_status_t stream_flags(uint32_t** p, int count, cudaStream_t s);
 // Clears every stream's flags of the current device (after a bounded wait has
 // given up, a flag may have been left raised).  The device must be idle.

@@ -112,15 +112,20 @@ void scratch_free(void* p, cudaStream_t s) {
 
 namespace {
 constexpr int kStreamFlagWords = 4096;
+constexpr size_t kMaxFlagStreams = 1024;
 struct StreamFlags {
     int device;
-    cudaStream_t stream;
+    unsigned long long id;
     uint32_t* words;
 };
 std::mutex g_flags_mu;
-std::vector<StreamFlags> g_flags;  // kept for the life of the process (16 KB per stream used)
+std::vector<StreamFlags> g_flags;  // kept for the life of the process (16 KB per stream used), newest last
 }  // namespace
 
+// Keyed by the stream's id, not by its handle: cudaStreamPerThread is one handle for
+// another stream in every host thread, and the handle of a destroyed stream comes back while
+// that stream's work may still run.  Launches on two streams must not share words: each would
+// take the other's parts for its own.
 nq_status_t stream_flags(uint32_t** p, int count, cudaStream_t s) {
     *p = nullptr;
     if (count > kStreamFlagWords) return fail(NQ_ERROR_INVALID_VALUE, "stream flags: too many words requested");
@@ -129,12 +134,17 @@ nq_status_t stream_flags(uint32_t** p, int count, cudaStream_t s) {
     if (cs != cudaStreamCaptureStatusNone) return NQ_SUCCESS;
     int dev = -1;
     NQ_CHECK_CUDA(cudaGetDevice(&dev), "cudaGetDevice");
+    unsigned long long id = 0;
+    NQ_CHECK_CUDA(cudaStreamGetId(s, &id), "cudaStreamGetId");
     std::lock_guard<std::mutex> lk(g_flags_mu);
-    for (const auto& f : g_flags)
-        if (f.device == dev && f.stream == s) {
-            *p = f.words;
+    for (auto f = g_flags.rbegin(); f != g_flags.rend(); ++f)
+        if (f->device == dev && f->id == id) {
+            *p = f->words;
             return NQ_SUCCESS;
         }
+    // A program that makes streams without end takes per-launch flags (the
+    // caller's memset) on those behind the first kMaxFlagStreams.
+    if (g_flags.size() >= kMaxFlagStreams) return NQ_SUCCESS;
     uint32_t* w = nullptr;
     if (cudaMalloc(&w, kStreamFlagWords * sizeof(uint32_t)) != cudaSuccess) {
         // e.g. another thread is capturing a graph in global mode: the caller
@@ -147,7 +157,7 @@ nq_status_t stream_flags(uint32_t** p, int count, cudaStream_t s) {
         cudaFree(w);
         return cuda_status(e, "cudaMemsetAsync(stream flags)");
     }
-    g_flags.push_back({dev, s, w});
+    g_flags.push_back({dev, id, w});
     *p = w;
     return NQ_SUCCESS;
 }

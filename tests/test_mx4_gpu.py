@@ -590,3 +590,68 @@ def test_first_call_of_a_thread(nq, m, n, k):
         t.join(60)
     torch.cuda.synchronize()
     assert not failed and torch.equal(out, ref) and torch.equal(*outs)
+
+
+def shared_out_operands(nq, m, n, k):
+    """Quantized operands of a product whose k-blocks are shared out over the CTAs."""
+    import torch
+    ops = []
+    for rows, seed in ((m, 2), (n, 1)):
+        q = buffers(nq, rows, k, R.NV, 0)
+        x = make(rows, k, seed, True, 0.1)
+        nq.quantize_rows_mx4(x.data_ptr(), nq.BF16, 0, q[0].data_ptr(), q[1].data_ptr(), q[2].data_ptr(), rows, k, R.NV,
+                             torch.cuda.current_stream().cuda_stream)
+        ops.append((q[0], q[1], q[2][:rows].contiguous()))
+    torch.cuda.synchronize()
+    return ops
+
+
+def test_shared_out_product_on_the_per_thread_stream(nq):
+    """cudaStreamPerThread is one handle and another stream in every thread: two threads that pass it share no flags."""
+    import threading
+    import torch
+    m, n, k = 4, 4096, 28672
+    a, b = shared_out_operands(nq, m, n, k)
+    ref = product(nq, a, b, m, n, k, R.NV, False)
+    outs = [[torch.full_like(ref, 99.0) for _ in range(40)] for _ in range(2)]
+    torch.cuda.synchronize()
+    failed, both = [], threading.Barrier(2)
+
+    def work(mine):
+        try:
+            both.wait(60)
+            for o in mine:
+                product(nq, a, b, m, n, k, R.NV, False, out=o, stream=2)   # cudaStreamPerThread
+            torch.cuda.synchronize()
+        except Exception as e:
+            failed.append(repr(e))
+
+    threads = [threading.Thread(target=work, args=(o,)) for o in outs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(120)
+    torch.cuda.synchronize()
+    assert not failed and all(torch.equal(o, ref) for mine in outs for o in mine)
+    assert nq.device_error_flags() == 0
+
+
+def test_shared_out_product_on_streams_without_end(nq):
+    """Streams destroyed with their work in flight, whose handles come back: every one counts as a new one; behind the
+    first thousand a launch brings its own flags."""
+    import torch
+    m, n, k = 2, 512, 16384
+    a, b = shared_out_operands(nq, m, n, k)
+    ref = product(nq, a, b, m, n, k, R.NV, False)
+    outs = [torch.full_like(ref, 99.0) for _ in range(1200)]
+    torch.cuda.synchronize()
+    rt, handles = torch.cuda.cudart(), set()
+    for o in outs:
+        h = C.c_void_p()
+        assert int(rt.cudaStreamCreate(C.addressof(h))) == 0
+        handles.add(h.value)
+        product(nq, a, b, m, n, k, R.NV, False, out=o, stream=h.value)
+        assert int(rt.cudaStreamDestroy(h.value)) == 0
+    torch.cuda.synchronize()
+    assert len(handles) < len(outs)   # (handles did come back)
+    assert all(torch.equal(o, ref) for o in outs) and nq.device_error_flags() == 0
