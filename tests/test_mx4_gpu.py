@@ -655,3 +655,29 @@ def test_shared_out_product_on_streams_without_end(nq):
     torch.cuda.synchronize()
     assert len(handles) < len(outs)   # (handles did come back)
     assert all(torch.equal(o, ref) for o in outs) and nq.device_error_flags() == 0
+
+
+# several 256 x 256 tiles a cluster (74 of them on 148 SMs): whole rounds and a tail of half tiles (171 tiles), a
+# remainder of more than half the clusters (112, ragged, rows of the output not whole 16 bytes), more than one band of
+# 32 row tiles (165), more than two rounds with a short K (285)
+MANY_TILES = [(2304, 4864, 600), (1700, 4001, 2100), (8400, 1100, 320), (3700, 4700, 40)]
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("bf16", [True, False])
+@pytest.mark.parametrize("shape", MANY_TILES)
+def test_product_of_many_tiles(nq, fmt, bf16, shape):
+    """Accumulators, scale words and stages handed from tile to tile; the same again, bit for bit."""
+    import torch
+    m, n, k = shape
+    a, va = operand(m, k, fmt, m + k)
+    b, vb = operand(n, k, fmt, n + k + 1, 0.05)
+    bias = torch.randn(n, device="cuda")
+    got = product(nq, a, b, m, n, k, fmt, bf16, 0.75, bias)
+    check_product(got, va, vb, a, b, k, bf16, 0.75, bias)
+    for _ in range(3):
+        assert torch.equal(product(nq, a, b, m, n, k, fmt, bf16, 0.75, bias), got)
+    plain = (a[0], a[1], None), (b[0], b[1], None)
+    got = product(nq, *plain, m, n, k, fmt, bf16)
+    check_product(got, va, vb, *plain, k, bf16)
+    assert nq.device_error_flags() == 0
