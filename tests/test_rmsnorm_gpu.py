@@ -556,3 +556,62 @@ def test_backward_of_rows_whose_sums_overflow(nq, bf16, shape, scale, dscale):
     dy, ds = rand(rows, cols, 3, bf16, dscale), rand(rows, cols, 4, bf16, dscale / scale)
     for d in (None, ds):
         check_backward(nq, h, w, dy, d, EPS)
+
+
+# many aligned rows: every block takes several of them through its ring
+RING_SHAPES = [(True, 2500, 2048), (True, 1300, 8192), (True, 700, 1032), (True, 3000, 4096), (False, 1500, 1000),
+               (False, 2000, 2048), (False, 700, 8192)]
+
+
+@pytest.mark.parametrize("bf16,rows,cols", RING_SHAPES)
+def test_many_rows(nq, bf16, rows, cols):
+    """Every output of many aligned rows, with and without the residual, against the 64-bit reference."""
+    import torch
+    x, res = rand(rows, cols, 1, bf16), rand(rows, cols, 2, bf16, 3.0)
+    w = rand(1, cols, 3, bf16).view(-1) + 1.0
+    x[rows // 2], res[rows // 2] = 0.0, 0.0
+    for r_ in (res, None):
+        s = torch.empty_like(x) if r_ is not None else None
+        h = reference_h(x, r_)
+        t, r = R.rmsnorm(h, w.double().cpu().numpy(), EPS)
+        for fmt in (E4M3, E5M2, INT8):
+            y, codes, _, scales = run(nq, x, r_, w, fmt, sum=s)
+            check_codes8(codes, scales, t, r, cols, fmt, exact=bf16)
+            check_y(y, t, r, cols)
+            assert s is None or np.array_equal(s.double().cpu().numpy(), h)
+        for fmt in (R.MX, R.NV):
+            y, codes, bs, g = run(nq, x, r_, w, fmt, four=True, sum=s)
+            check_mx4(nq, (codes, bs, g), t, r, rows, cols, fmt)
+            check_y(y, t, r, cols)
+    assert nq.device_error_flags() == 0
+
+
+@pytest.mark.parametrize("bf16,rows,cols", [(True, 2500, 2048), (True, 1300, 8192), (False, 2000, 2048)])
+def test_many_rows_in_place_and_in_pieces(nq, bf16, rows, cols):
+    """The sum written over an input while the rows behind it are on their way in; and the same rows in calls of a
+    few hundred, which another kernel takes: equal codes (they do not depend on the order of a sum), scales within
+    both sums' tolerance."""
+    import torch
+    x, res = rand(rows, cols, 1, bf16), rand(rows, cols, 2, bf16, 3.0)
+    w = rand(1, cols, 3, bf16).view(-1) + 1.0
+    s = torch.empty_like(x)
+    y, codes, _, scales = run(nq, x, res, w, E4M3, sum=s)
+    _, nv, nvb, nvg = run(nq, x, res, w, R.NV, four=True, sum=s)
+    for k in range(2):
+        a, b = x.clone(), res.clone()
+        y2, c2, _, s2 = run(nq, a, b, w, E4M3, sum=(a, b)[k])
+        assert torch.equal((a, b)[k], s) and torch.equal((b, a)[k], (res, x)[k])
+        assert torch.equal(y2, y) and torch.equal(c2, codes) and torch.equal(s2, scales)
+    pitch, words = nq.mx4_row_bytes(cols), R.words(cols, R.NV)
+    for at in range(0, rows, 512):   # whole tiles of scales
+        part = slice(at, min(rows, at + 512))
+        n = part.stop - at
+        ps = torch.empty_like(x[part])
+        _, c2, _, s2 = run(nq, x[part], res[part], w, E4M3, sum=ps)
+        assert torch.equal(c2, codes[part]) and torch.equal(ps, s[part])
+        assert torch.all((s2.double() / scales[part].double() - 1).abs() <= 2 * tol_r(cols) + 8 * U)
+        _, c4, b4, g4 = run(nq, x[part], res[part], w, R.NV, four=True)
+        idx = torch.from_numpy(R.scale_index(n, cols, R.NV)).cuda()
+        assert torch.equal(c4, nv[at * pitch:part.stop * pitch]) and torch.equal(b4[idx], nvb[at // 128 * words * 512:][idx])
+        assert torch.all((g4.double() / nvg[part].double() - 1).abs() <= 2 * tol_r(cols) + 8 * U)
+    assert nq.device_error_flags() == 0
