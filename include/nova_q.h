@@ -441,7 +441,7 @@ typedef struct {
     int rows, cols;
     nq_dtype_t dtype;        /* of x, residual, sum, y and gradients: NQ_F32 or NQ_BF16 */
     nq_dtype_t weight_dtype; /* NQ_F32 or NQ_BF16 */
-    float eps;               /* >= 0 */
+    float eps;               /* at least FLT_MIN, finite: squares that fp32 loses then do not count beside it */
     int x_stride;            /* elements between rows of x; 0 = cols */
     int residual_stride;     /* elements between rows of residual; 0 = cols */
 } nq_rmsnorm_desc_t;

@@ -966,7 +966,7 @@ nq_status_t check_desc(const char* who, const nq_rmsnorm_desc_t* d, size_t* xs, 
     if (d->cols > (1 << 30)) return fail(NQ_ERROR_UNSUPPORTED, std::string(who) + ": more than 2^30 columns");
     if (d->dtype != NQ_F32 && d->dtype != NQ_BF16) return bad(who, "dtype must be NQ_F32 or NQ_BF16");
     if (d->weight_dtype != NQ_F32 && d->weight_dtype != NQ_BF16) return bad(who, "weight_dtype must be NQ_F32 or NQ_BF16");
-    if (!(d->eps > 0.0f) || !(d->eps <= FLT_MAX)) return bad(who, "eps must be positive and finite");
+    if (!(d->eps >= FLT_MIN) || !(d->eps <= FLT_MAX)) return bad(who, "eps must be at least FLT_MIN (1.18e-38) and finite");
     if ((d->x_stride && d->x_stride < d->cols) || (d->residual_stride && d->residual_stride < d->cols))
         return bad(who, "a row stride is smaller than cols");
     *xs = d->x_stride ? d->x_stride : d->cols;

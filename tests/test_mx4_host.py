@@ -155,3 +155,19 @@ def test_rmsnorm_backward_refusals(nq):
     for bad in (dict(rows=-1), dict(eps=0.0), dict(dtype=2), dict(x_stride=2)):
         assert call(**bad) == 1, bad
     assert call(dict(h=None), cols=0) == 0 and call(dict(h=None, dw=None), rows=0) == 0
+
+
+def test_rmsnorm_eps_range(nq):
+    """eps from FLT_MIN to FLT_MAX, as the header says: squares below fp32's range would count beside a smaller one."""
+    smallest = float(np.finfo(np.float32).tiny)
+    for eps in (smallest, 1e-5, 1.0, float(np.finfo(np.float32).max)):
+        d = nq.make_rmsnorm_desc(0, 64, eps=eps)
+        assert nq.rmsnorm_quantize.raw(C.byref(d), P, None, P, None, P + 4096, None, None, nq.E4M3, None) == 0
+        assert nq.rmsnorm_quantize_mx4.raw(C.byref(d), P, None, P, None, P + 4096, None, None, None, nq.NVFP4, None) == 0
+        assert nq.rmsnorm_backward.raw(C.byref(d), P, P, P, None, P + 4096, None, None) == 0
+    for eps in (0.0, 1e-45, 1e-39, 0.5 * smallest):
+        d = nq.make_rmsnorm_desc(4, 64, eps=eps)
+        for call in (lambda: nq.rmsnorm_quantize.raw(C.byref(d), P, None, P, None, P + 4096, None, None, nq.E4M3, None),
+                     lambda: nq.rmsnorm_quantize_mx4.raw(C.byref(d), P, None, P, None, P + 4096, None, None, None, nq.NVFP4, None),
+                     lambda: nq.rmsnorm_backward.raw(C.byref(d), P, P, P, None, P + 4096, None, None)):
+            assert call() == 1 and b"eps" in nq.lib.nq_last_error()
