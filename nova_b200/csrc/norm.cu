@@ -1021,7 +1021,8 @@ nq_status_t launch_norm(const NormArgs& a, const DeviceInfo& di, cudaStream_t s,
             const int cut = nvec + 1;  // a row may begin inside its first vector
             if (cut <= 256) return launch_norm_cut<In, OUT, 1, true>(a, (cut + 31) / 32 * 32, di, s, who);
             const int threads = ((cut + NVMAX - 1) / NVMAX + 31) / 32 * 32;
-            if (sizeof(In) == 4 && threads <= 320) return launch_norm_cut<In, OUT, NVMAX, true>(a, threads, di, s, who);
+            if constexpr (sizeof(In) == 4)
+                if (threads <= 320) return launch_norm_cut<In, OUT, NVMAX, true>(a, threads, di, s, who);
             return launch_norm_cut<In, OUT, NVMAX, false>(a, threads, di, s, who);
         }
     }
