@@ -64,7 +64,8 @@ __global__ void __launch_bounds__(256) k_mx4_empty(int M, int N, MxEpi ep) {
 
 // ---------------- CTA pair, 256 x 256 tiles ----------------
 // Bound by the tensor pipe and, run back to back, by the board's power: 4096^3
-// MXFP4 27.4 us (5.0 PFLOP/s), 8192^3 NVFP4 194 us (5.7 PFLOP/s, tensor pipe 74%
+// MXFP4 27.4 us (5.0 PFLOP/s) on operands that stay in L2, 30.2 on changing ones, 34.8 for seconds on
+// end at 1.61 GHz; 8192^3 NVFP4 194 us (5.7 PFLOP/s, tensor pipe 74%
 // active, DRAM traffic 211 MB of 210), 8192 x 14336 x 4096 NVFP4 218 us (4.4
 // PFLOP/s) for seconds on end, with SM clocks at 1.46 GHz under the cap.  Of those
 // 218 us the operands' way into shared memory and the epilogue take about 30 each

@@ -10,11 +10,11 @@
 //
 // Which kernel: rows in registers (k_norm_rows: a warp or a block a row); many
 // aligned rows through a bulk-copy ring (k_norm_ring: 16384 x 8192 bf16 with
-// residual, E4M3: 154 us, 6.1 TB/s, against 165 from registers; 16384 columns lose
-// by it, 298 against 286); dense rows of odd widths cut where memory is (k_norm_cut: 16384 x 5003 bf16 130 us
-// against 187); rows too wide for registers in two passes.  One row: 2.6 us a launch
-// in a graph.  The gradient: 8192 x 4096 bf16 51 us (5.2 TB/s), of which the partial
-// rows' sum takes 4.5.
+// residual, E4M3: 153 us, 6.1 TB/s, against 165 from registers, in a graph of passes; to NVFP4 237, bound
+// by the encode's arithmetic; 16384 columns lose by it, 298 against 285); dense rows of odd widths cut where
+// memory is (k_norm_cut: 16384 x 5003 bf16 120 us against 187); rows too wide for
+// registers in two passes.  One row: 2.7 us a launch in a graph.  The gradient: 8192 x 4096
+// bf16 51 us (5.2 TB/s), of which the partial rows' sum takes 4.5; 4096 x 16384 bf16 160, fp32 326.
 #include <algorithm>
 #include <cfloat>
 #include <mutex>
@@ -1113,7 +1113,7 @@ nq_status_t launch_grad(const GradArgs& a, float* dw, const DeviceInfo& di, cuda
     int stages = 0;
     size_t smem = 0;
     if (VEC) {
-        // two to four rows ahead, about 40 KB of them a block
+        // two to four rows ahead, up to 60 KB of them a block, or two rows where those are more
         // (room for dsum even where dx is not asked for: the grid, and with it the order of
         // the weight gradient's sum, does not depend on dx)
         const size_t row = static_cast<size_t>(a.cols) * sizeof(In) * (a.dsum ? 3 : 2);
