@@ -615,3 +615,35 @@ def test_many_rows_in_place_and_in_pieces(nq, bf16, rows, cols):
         assert torch.equal(c4, nv[at * pitch:part.stop * pitch]) and torch.equal(b4[idx], nvb[at // 128 * words * 512:][idx])
         assert torch.all((g4.double() / nvg[part].double() - 1).abs() <= 2 * tol_r(cols) + 8 * U)
     assert nq.device_error_flags() == 0
+
+
+@pytest.mark.parametrize("bf16", [True, False])
+@pytest.mark.parametrize("shape", FAR_SHAPES)
+def test_far_rows_in_place_and_rows_beside_them(nq, bf16, shape):
+    """A row whose squares overflow with the sum over either input, or with a weight of the other type: the results of
+    separate tensors; the rows beside it are those of a call without it."""
+    import torch
+    rows, cols = shape
+    x, res = rand(rows, cols, 1, bf16), rand(rows, cols, 2, bf16)
+    w = rand(1, cols, 3, not bf16).view(-1).clamp(-0.4, 0.4) + 1.0
+    calm = run(nq, x, res, w, E4M3)
+    x[rows - 1, 2:70] = 1e25
+    s = torch.empty_like(x)
+    far = run(nq, x, res, w, E4M3, sum=s)
+    nv = run(nq, x, res, w, R.NV, four=True)
+    mx = run(nq, x, res, w, R.MX, four=True)
+    t, r = product32(reference_h(x, res), w.double().cpu().numpy()), R.rmsnorm(reference_h(x, res), 1.0, EPS)[1]
+    check_codes8(far[1], far[3], t, r, cols, E4M3)
+    check_mx4(nq, nv[1:], t, r, rows, cols, R.NV)
+    check_mx4(nq, mx[1:], t, r, rows, cols, R.MX)
+    for a, b in ((calm[0], far[0]), (calm[1], far[1]), (calm[3], far[3])):
+        assert torch.equal(a[:rows - 1], b[:rows - 1])
+    for k in range(2):
+        a, b = x.clone(), res.clone()
+        y, codes, _, scales = run(nq, a, b, w, E4M3, sum=(a, b)[k])
+        assert torch.equal((a, b)[k], s) and torch.equal(y, far[0]) and torch.equal(codes, far[1]) and torch.equal(scales, far[3])
+        for fmt, want in ((R.NV, nv), (R.MX, mx)):
+            a, b = x.clone(), res.clone()
+            y, codes, bs, g = run(nq, a, b, w, fmt, four=True, sum=(a, b)[k])
+            assert torch.equal(y, want[0]) and torch.equal(codes, want[1]) and torch.equal(bs, want[2])
+            assert g is None or torch.equal(g, want[3])
